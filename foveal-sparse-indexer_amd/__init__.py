@@ -42,6 +42,7 @@ from .attention import (
     triton_foveal_sparse_attention,
     triton_fused_sram_indexer_attention,
 )
+from .sink_attention import sink_window_attention
 from .block_matmul import (
     BlockSparseLinear,
     BlockwiseMatMul2D,
@@ -77,6 +78,7 @@ __all__ = [
     "decode_attention",
     "decode_step_attention",
     "sparse_attention",
+    "sink_window_attention",
     "triton_foveal_sparse_attention",
     "triton_fused_sram_indexer_attention",
     "sram_indexer_attention",

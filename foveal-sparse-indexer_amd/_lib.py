@@ -7,6 +7,7 @@ the HIP library is not built or not loadable.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import os
@@ -32,6 +33,8 @@ FSI_ERR_WORKSPACE = -8
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
 DTYPE_F16 = 2  # fsi_sram_indexer_attention only
+
+KV_FORMATS = {None: 0, "mxfp8": 1, "mxfp4": 2}  # fsi_kv_format; None: the cache's own bf16 pages
 
 ACTIVATIONS = {"swiglu": 0, "silu": 1, "gelu": 2, "relu": 3, "relu2": 4}
 ROUNDING = {"eager": 0, "fused": 1, "fp32": 2}
@@ -164,6 +167,23 @@ SIGNATURES: dict[str, tuple] = {
         [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_i64,
          _c_i64, _c_i64, _c_i64, ctypes.c_float, _c_ptr, _c_ptr, _c_ptr],
     ),
+    "fsi_kv_mx_block_bytes": (_c_i64, [_c_i64, _c_int]),
+    "fsi_kv_mx_write": (
+        _c_int,
+        [_c_ptr, _c_ptr] + [_c_i64] * 10 + [_c_int, _c_int, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr,
+                                            _c_ptr, _c_ptr],
+    ),
+    "fsi_kv_mx_read": (
+        _c_int,
+        [_c_ptr, _c_ptr, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_int, _c_ptr, _c_ptr,
+         _c_ptr],
+    ),
+    "fsi_decode_attn_sinks_workspace_size": (_c_size, [_c_i64] * 4 + [_c_int] + [_c_i64] * 4),
+    "fsi_decode_attn_sinks": (
+        _c_int,
+        [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr,
+         _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_float, _c_ptr, _c_ptr, _c_size, _c_ptr, _c_ptr],
+    ),
     "fsi_sparse_attn_workspace_size": (_c_size, [_c_i64, _c_i64, _c_i64, _c_i64]),
     "fsi_decode_attn_bwd_q": (
         _c_int,
@@ -183,6 +203,17 @@ SIGNATURES: dict[str, tuple] = {
          _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i64,
          _c_ptr, _c_i64, _c_i64, ctypes.c_float, _c_int, _c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr, _c_size,
          _c_ptr, _c_ptr],
+    ),
+    "fsi_sink_attn": (
+        _c_int,
+        [_c_ptr, _c_i64, _c_i64, _c_i64] * 3 + [_c_i64] * 8 + [_c_ptr, ctypes.c_float, _c_int, _c_ptr, _c_i64, _c_i64,
+                                                             _c_i64, _c_ptr, _c_ptr],
+    ),
+    "fsi_sink_attn_bwd_workspace_size": (_c_size, [_c_i64] * 8),
+    "fsi_sink_attn_bwd": (
+        _c_int,
+        [_c_ptr, _c_i64, _c_i64, _c_i64] * 5 + [_c_ptr] + [_c_i64] * 8
+        + [_c_ptr, ctypes.c_float, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_size, _c_ptr],
     ),
     "fsi_sram_indexer_attention": (
         _c_int,
@@ -337,6 +368,12 @@ def dtype_code(dt: torch.dtype, what: str) -> int:
 def stream_handle(device: torch.device) -> int:
     index = device.index
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
+
+def device_guard(device: torch.device):
+    """Context in which `device` is the current one (a launch goes to the current device)."""
+    same = device.index is None or device.index == torch.cuda.current_device()
+    return contextlib.nullcontext() if same else torch.cuda.device(device)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -127,6 +127,14 @@ class FovealKVCache:
       * contiguous (every other dtype / page size / head_dim, or paged=False):
         `k_cache` / `v_cache` are (B, Hkv, max_seq_len, head_dim) exactly as in
         the reference, so callers may read and write them directly.
+    kv_format "mxfp8" or "mxfp4" holds K and V of the paged layout in 8 or 4 bits
+    instead: 32 dims of a token and head share a power of two 2^e, the values are e4m3
+    (up to 448) or e2m1 (up to 6), rounded to nearest even as they are written, with e the
+    smallest integer that keeps the group's largest |x| within half a step above the
+    largest value (0.53 or 1.03 bytes an element with the scale; an infinity or NaN makes
+    its group read as NaN).  K and V are given and read back in `dtype` (bfloat16 or
+    float32; page_size 64, head_dim 64, 96, 128 or 256), the 16-D page state stays as it is,
+    and decode_attention reads the pages as they are held.
     """
 
     def __init__(
@@ -142,14 +150,24 @@ class FovealKVCache:
         n_phys_pages: Optional[int] = None,
         page_table: Optional[Tensor] = None,
         paged: Optional[bool] = None,
+        kv_format: Optional[str] = None,
     ):
+        if kv_format not in _lib.KV_FORMATS:
+            raise ValueError(f"FovealKVCache: kv_format {kv_format!r} (None, 'mxfp8' or 'mxfp4')")
         if dtype not in (torch.float32, torch.bfloat16):
             raise TypeError(f"FovealKVCache: dtype {dtype} unsupported (float32 or bfloat16)")
         if page_size <= 0 or head_dim <= 0 or head_dim > 256:
             raise ValueError(f"FovealKVCache: page_size {page_size} / head_dim {head_dim} unsupported")
-        pageable = dtype == torch.bfloat16 and page_size == PAGE_SIZE and head_dim in (64, 128)
-        if paged and not pageable:
-            raise ValueError("FovealKVCache: the paged layout needs bfloat16, page_size 64 and head_dim 64 or 128")
+        if kv_format is not None:
+            pageable = page_size == PAGE_SIZE and head_dim in (64, 96, 128, 256)
+            if not pageable or paged is False:
+                raise ValueError(f"FovealKVCache: kv_format {kv_format!r} needs the paged layout, page_size 64 and "
+                                 "head_dim 64, 96, 128 or 256")
+        else:
+            pageable = dtype == torch.bfloat16 and page_size == PAGE_SIZE and head_dim in (64, 128)
+            if paged and not pageable:
+                raise ValueError("FovealKVCache: the paged layout needs bfloat16, page_size 64 and head_dim 64 or 128")
+        self.kv_format = kv_format
         self.paged = pageable if paged is None else bool(paged)
         if not self.paged and (page_table is not None or n_phys_pages is not None):
             raise ValueError("FovealKVCache: page_table / n_phys_pages apply to the paged layout only")
@@ -171,9 +189,13 @@ class FovealKVCache:
                 raise ValueError(f"FovealKVCache: page table {tuple(self.page_table.shape)} != "
                                  f"{(batch_size, self.max_pages)}")
             self.n_phys_pages = int(n_phys_pages) if n_phys_pages is not None else batch_size * self.max_pages
-            per_page = num_kv_heads * page_size * head_dim
-            self.k_cache = torch.zeros(self.n_phys_pages, per_page, device=self.device, dtype=dtype)
-            self.v_cache = torch.zeros(self.n_phys_pages, per_page, device=self.device, dtype=dtype)
+            if kv_format is None:
+                per_page, held = num_kv_heads * page_size * head_dim, dtype
+            else:
+                per_page = num_kv_heads * _lib.lib().fsi_kv_mx_block_bytes(head_dim, _lib.KV_FORMATS[kv_format])
+                held = torch.uint8
+            self.k_cache = torch.zeros(self.n_phys_pages, per_page, device=self.device, dtype=held)
+            self.v_cache = torch.zeros(self.n_phys_pages, per_page, device=self.device, dtype=held)
         else:
             self.page_table = None
             self.n_phys_pages = 0
@@ -187,12 +209,20 @@ class FovealKVCache:
         self.seq_len = 0
         self.completed_pages = 0
 
-    def _write(self, k: Tensor, v: Tensor, start: int) -> None:
+    def _write(self, k: Tensor, v: Tensor, start: int | Tensor) -> None:
         what = "FovealKVCache"
         B, H, n, hd = k.shape
         if (B, H, hd) != (self.batch_size, self.num_kv_heads, self.head_dim) or v.shape != k.shape:
             raise ValueError(f"{what}: K {tuple(k.shape)} / V {tuple(v.shape)} do not match the cache")
-        if start < 0 or start + n > self.max_seq_len:
+        rows = None
+        if isinstance(start, Tensor):
+            if self.kv_format is None:
+                raise TypeError(f"{what}: per-sequence start positions need a cache with a kv_format")
+            rows = start.to(device=self.k_cache.device, dtype=torch.int32).reshape(-1).contiguous()
+            if rows.numel() != B:
+                raise ValueError(f"{what}: {rows.numel()} start positions for {B} sequences")
+            start = 0
+        elif start < 0 or start + n > self.max_seq_len:
             raise RuntimeError(f"KV cache capacity {self.max_seq_len} exceeded.")
         if not self.paged:
             # the reference layout: a slice copy (attention.py:72-73), cast to the cache dtype
@@ -207,6 +237,10 @@ class FovealKVCache:
         if v.stride(-1) != 1:
             v = v.contiguous()
         _lib.require_gpu(k, v, self.k_cache, what=what)
+        if self.kv_format is not None:
+            _kv_mx_write_op(k.detach(), v.detach(), _lib.KV_FORMATS[self.kv_format], rows, int(start),
+                            self.page_table, self.max_pages, self.n_phys_pages, self.k_cache, self.v_cache)
+            return
         _kv_write_op(k, v, int(start), self.page_table, self.max_pages, self.n_phys_pages, self.k_cache, self.v_cache)
 
     def update(self, k_step: Tensor, v_step: Tensor, ki_step: Tensor, vi_step: Tensor) -> int:
@@ -226,9 +260,11 @@ class FovealKVCache:
         self.seq_len += 1
         return pos
 
-    def load_dense(self, k: Tensor, v: Tensor, start: int = 0) -> None:
+    def load_dense(self, k: Tensor, v: Tensor, start: int | Tensor = 0) -> None:
         """Write (B, Hkv, n, hd) K/V at positions start .. start + n - 1 (the
-        reference layout) without touching the 16-D page state."""
+        reference layout) without touching the 16-D page state.  With a kv_format,
+        start may be a (B,) integer tensor, one position per sequence; tokens outside the
+        cache are then skipped and reported as the other device-side index errors are."""
         self._write(k, v, start)
 
     def to_dense(self, n_tok: Optional[int] = None, batch: Optional[slice] = None):
@@ -239,6 +275,10 @@ class FovealKVCache:
             sel = batch if batch is not None else slice(None)
             return self.k_cache[sel, :, :n].clone(), self.v_cache[sel, :, :n].clone()
         rows = self.page_table[batch] if batch is not None else self.page_table
+        if self.kv_format is not None:
+            return _kv_mx_read_op(self.k_cache, self.v_cache, rows.contiguous(), _lib.KV_FORMATS[self.kv_format],
+                                  self.num_kv_heads, n, self.head_dim, self.max_pages, self.n_phys_pages,
+                                  _lib.dtype_code(self.dtype, "FovealKVCache.to_dense"))
         return _kv_read_op(self.k_cache, self.v_cache, rows.contiguous(), self.num_kv_heads, n, self.head_dim,
                            self.max_pages, self.n_phys_pages)
 
@@ -290,6 +330,49 @@ def _kv_read_op(k_cache: Tensor, v_cache: Tensor, rows: Tensor, heads: int, n: i
     return k, v
 
 
+@_lib.fsi_op("kv_mx_write", lambda k, v, fmt, rows, start, page_table, max_pages, n_phys, k_cache, v_cache: None,
+             mutates_args=("k_cache", "v_cache"))
+def _kv_mx_write_op(k: Tensor, v: Tensor, fmt: int, rows: Optional[Tensor], start: int, page_table: Tensor,
+                    max_pages: int, n_phys: int, k_cache: Tensor, v_cache: Tensor) -> None:
+    """fsi_kv_mx_write: (B, H, n, hd) K/V at positions rows[b] (or start) .. into 8- or 4-bit pages."""
+    what = "FovealKVCache"
+    dev = k.device
+    B, H, n, hd = k.shape
+    err = _lib.error_word(dev)
+    with _lib.device_guard(dev):
+        st = _lib.lib().fsi_kv_mx_write(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
+                                        v.stride(0), v.stride(1), v.stride(2), B, H, n, hd,
+                                        _lib.dtype_code(k.dtype, what), fmt, _lib.ptr(rows), start,
+                                        page_table.data_ptr(), max_pages, n_phys, k_cache.data_ptr(),
+                                        v_cache.data_ptr(), err.data_ptr(), _lib.stream_handle(dev))
+    _lib.check(st, what)
+    if _lib.checks_enabled():
+        _lib.raise_device_errors(dev, what)
+
+
+_CODE_DTYPES = {_lib.DTYPE_F32: torch.float32, _lib.DTYPE_BF16: torch.bfloat16}
+
+
+def _kv_mx_read_fake(k_cache, v_cache, rows, fmt, heads, n, hd, max_pages, n_phys, dtype):
+    k = k_cache.new_empty((rows.shape[0], heads, n, hd), dtype=_CODE_DTYPES[dtype])
+    return k, torch.empty_like(k)
+
+
+@_lib.fsi_op("kv_mx_read", _kv_mx_read_fake)
+def _kv_mx_read_op(k_cache: Tensor, v_cache: Tensor, rows: Tensor, fmt: int, heads: int, n: int, hd: int,
+                   max_pages: int, n_phys: int, dtype: int) -> Tuple[Tensor, Tensor]:
+    """fsi_kv_mx_read: positions [0, n) of the sequences whose page-table rows are given, (b, H, n, hd)."""
+    dev = k_cache.device
+    k = torch.empty((rows.shape[0], heads, n, hd), dtype=_CODE_DTYPES[dtype], device=dev)
+    v = torch.empty_like(k)
+    with _lib.device_guard(dev):
+        st = _lib.lib().fsi_kv_mx_read(k_cache.data_ptr(), v_cache.data_ptr(), fmt, rows.shape[0], heads, n, hd,
+                                       rows.data_ptr(), max_pages, n_phys, dtype, k.data_ptr(), v.data_ptr(),
+                                       _lib.stream_handle(dev))
+    _lib.check(st, "FovealKVCache.to_dense")
+    return k, v
+
+
 def _decode_launch(q3: Tensor, k_cache: Tensor, v_cache: Tensor, page_table: Optional[Tensor], max_pages: int,
                    n_phys: int, max_seq_len: int, page_size: int, n_kv_heads: int, pos_rows: Optional[Tensor],
                    pos_val: int, window: int, remote_pages: Optional[Tensor], remote_counts: Optional[Tensor],
@@ -332,6 +415,42 @@ def _decode_op(q3: Tensor, k_cache: Tensor, v_cache: Tensor, page_table: Optiona
     """Decode attention into a new (B, Hq, hd) tensor."""
     return _decode_launch(q3, k_cache, v_cache, page_table, max_pages, n_phys, max_seq_len, page_size, n_kv_heads,
                           pos_rows, pos_val, window, remote_pages, remote_counts, cap, scale, torch.empty_like(q3))
+
+
+def _decode_sinks_launch(q3: Tensor, k_cache: Tensor, v_cache: Tensor, fmt: int, page_table: Tensor, max_pages: int,
+                         n_phys: int, n_kv_heads: int, pos_rows: Optional[Tensor], pos_val: int, window: int,
+                         sinks: int, remote_pages: Optional[Tensor], remote_counts: Optional[Tensor], cap: int,
+                         scale: float, out: Tensor) -> Tensor:
+    """fsi_decode_attn_sinks.  Its partials come from the allocator, not from the stream's shared
+    workspace, so graphs captured on one stream may be replayed side by side."""
+    what = "decode_attention"
+    dev = q3.device
+    B, Hq, hd = q3.shape
+    L = _lib.lib()
+    err = _lib.error_word(dev)
+    need = L.fsi_decode_attn_sinks_workspace_size(B, Hq, n_kv_heads, hd, fmt, window, sinks, cap, max_pages)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    with _lib.device_guard(dev):
+        st = L.fsi_decode_attn_sinks(q3.data_ptr(), _lib.dtype_code(q3.dtype, what), k_cache.data_ptr(),
+                                     v_cache.data_ptr(), fmt, page_table.data_ptr(), max_pages, n_phys,
+                                     _lib.ptr(pos_rows), pos_val, window, sinks, _lib.ptr(remote_pages),
+                                     _lib.ptr(remote_counts), cap, B, Hq, n_kv_heads, hd, scale, out.data_ptr(),
+                                     _lib.ptr(ws), need, err.data_ptr(), _lib.stream_handle(dev))
+    _lib.check(st, what)
+    if _lib.checks_enabled():
+        _lib.raise_device_errors(dev, what)
+    return out
+
+
+@_lib.fsi_op("decode_attention_sinks", lambda q3, *rest: torch.empty_like(q3))
+def _decode_sinks_op(q3: Tensor, k_cache: Tensor, v_cache: Tensor, fmt: int, page_table: Tensor, max_pages: int,
+                     n_phys: int, n_kv_heads: int, pos_rows: Optional[Tensor], pos_val: int, window: int, sinks: int,
+                     remote_pages: Optional[Tensor], remote_counts: Optional[Tensor], cap: int,
+                     scale: float) -> Tensor:
+    """Decode attention with sinks, or over 8- or 4-bit pages, into a new (B, Hq, hd) tensor."""
+    return _decode_sinks_launch(q3, k_cache, v_cache, fmt, page_table, max_pages, n_phys, n_kv_heads, pos_rows,
+                                pos_val, window, sinks, remote_pages, remote_counts, cap, scale,
+                                torch.empty_like(q3))
 
 
 def _decode_step_fake(qi, kp, vp, completed, top_p, k_min, k_max, cap, want_ctx, q3, k_cache, v_cache, page_table,
@@ -383,8 +502,8 @@ def decode_step_attention(q: Tensor, qi: Tensor, cache: FovealKVCache, *, pos: i
     cap = max(K_max, K_min, 1); no autograd (use decode_route + decode_attention)."""
     what = "decode_step"
     dev = _lib.require_gpu(q, qi, cache.kp_cache, what=what)
-    if not cache.paged:
-        raise ValueError(f"{what}: the fused step needs the paged cache layout")
+    if not cache.paged or cache.kv_format is not None:
+        raise ValueError(f"{what}: the fused step needs the paged cache layout in bf16")
     B = q.shape[0]
     Hq, hd = q.shape[1], q.shape[-1]
     q3 = q.detach().reshape(B, Hq, hd).contiguous()
@@ -468,6 +587,34 @@ class _DecodeAttnFn(torch.autograd.Function):
         return dq.to(q3.dtype), None, None, None, None, None, None, None, None
 
 
+def _decode_attention_sinks(q3: Tensor, cache: FovealKVCache, pos_rows: Optional[Tensor], pos_val: int, window: int,
+                            sinks: int, remote_pages: Optional[Tensor], remote_counts: Optional[Tensor], cap: int,
+                            scale: float, out: Optional[Tensor]) -> Tensor:
+    what = "decode_attention"
+    if not cache.paged:
+        raise ValueError(f"{what}: sinks need the paged cache layout")
+    if torch.is_grad_enabled() and q3.requires_grad:
+        raise RuntimeError(f"{what}: no gradient for q with sinks or a kv_format; call under torch.no_grad()")
+    B = q3.shape[0]
+    if pos_rows is not None and pos_rows.numel() != B:
+        raise ValueError(f"{what}: {pos_rows.numel()} positions for {B} sequences")
+    if cap and (tuple(remote_pages.shape) != (B, cap) or remote_counts.numel() != B):
+        raise ValueError(f"{what}: pages {tuple(remote_pages.shape)} / counts {tuple(remote_counts.shape)} are not "
+                         f"(B, capacity) / (B,) for {B} sequences")
+    q3 = q3.detach().contiguous()
+    if q3.data_ptr() % 16:
+        q3 = q3.clone()
+    args = (cache.k_cache, cache.v_cache, _lib.KV_FORMATS[cache.kv_format], cache.page_table, cache.max_pages,
+            cache.n_phys_pages, cache.num_kv_heads, pos_rows, pos_val, window, sinks, remote_pages, remote_counts,
+            cap, scale)
+    if out is None:
+        return _decode_sinks_op(q3, *args)
+    if tuple(out.shape) != tuple(q3.shape) or out.dtype != q3.dtype or not out.is_contiguous():
+        raise ValueError(f"{what}: out must be a contiguous {tuple(q3.shape)} {q3.dtype} tensor")
+    _lib.require_gpu(q3, out, what=what)
+    return _decode_sinks_launch(q3, *args, out)
+
+
 def decode_attention(
     q: Tensor,
     cache: FovealKVCache,
@@ -478,12 +625,18 @@ def decode_attention(
     remote_counts: Optional[Tensor],
     scale: float,
     out: Optional[Tensor] = None,
+    sinks: int = 0,
 ) -> Tensor:
     """softmax(scale q K^T) V over [max(0, pos + 1 - window), pos] plus the
     selected remote pages, for every sequence and query head (attention.py:339-365).
     q: (B, Hq, hd) or (B, Hq, 1, hd) in the cache's dtype.  Returns (B, Hq, hd).
     Paged caches run the split-K MFMA kernels, contiguous ones the generic
-    kernel.  Differentiable in q (the cached keys and values are constants)."""
+    kernel.  Differentiable in q (the cached keys and values are constants).
+
+    sinks: the first tokens that stay visible beside the window (paged caches).  With sinks,
+    or over a cache with a kv_format, a token of several of sinks, window and pages counts
+    once, a sequence without any token gets 0, and there is no gradient: a q that would
+    need one is refused."""
     what = "decode_attention"
     dev = _lib.require_gpu(q, cache.k_cache, what=what)
     B = q.shape[0]
@@ -505,6 +658,11 @@ def decode_attention(
         cap = remote_pages.shape[-1]
     else:
         remote_pages = remote_counts = None
+    if sinks < 0:
+        raise ValueError(f"{what}: sinks {sinks} < 0")
+    if sinks or cache.kv_format is not None:
+        return _decode_attention_sinks(q3, cache, pos_rows, pos_val, int(window), int(sinks), remote_pages,
+                                       remote_counts, cap, float(scale), out)
     if torch.is_grad_enabled() and q3.requires_grad:
         res = _DecodeAttnFn.apply(q3.contiguous(), cache, pos_rows, pos_val, int(window), remote_pages,
                                   remote_counts, cap, float(scale))
@@ -973,8 +1131,10 @@ class FovealSparseAttention(nn.Module):
         page_mass = probs.view(batch, self.num_heads, num_pages, num_pages, self.page_size).sum(dim=-1)
         return page_mass.mean(dim=1)
 
-    def init_kv_cache(self, batch_size: int, max_seq_len: int, device: torch.device) -> FovealKVCache:
-        """A paged cache for decoding (attention.py:271-282)."""
+    def init_kv_cache(self, batch_size: int, max_seq_len: int, device: torch.device,
+                      kv_format: Optional[str] = None) -> FovealKVCache:
+        """A paged cache for decoding (attention.py:271-282); kv_format "mxfp8" or "mxfp4" holds
+        K and V in 8 or 4 bits (decode_step then runs without autograd only)."""
         return FovealKVCache(
             batch_size=batch_size,
             max_seq_len=max_seq_len,
@@ -984,6 +1144,7 @@ class FovealSparseAttention(nn.Module):
             page_size=self.page_size,
             device=device,
             dtype=self.q_proj.weight.dtype,
+            kv_format=kv_format,
         )
 
     def decode_step(self, x_step: Tensor, kv_cache: FovealKVCache) -> Tuple[Tensor, Dict[str, Any]]:
@@ -1003,7 +1164,7 @@ class FovealSparseAttention(nn.Module):
 
         completed = kv_cache.completed_pages
         want_ctx = self.use_additive_stream and completed > 0
-        fused = (kv_cache.paged and qi.dtype == torch.bfloat16
+        fused = (kv_cache.paged and kv_cache.kv_format is None and qi.dtype == torch.bfloat16
                  and not (torch.is_grad_enabled() and q.requires_grad))
         if fused:  # routing beside the local-window attention, one stream
             res = decode_step_attention(

@@ -1,0 +1,65 @@
+// Attention over a sliding window and the first tokens ("sinks"), forward and backward: the
+// parameters and the mask that the kernels of sink_attn.hip and sink_attn_bf16.hip share.
+//
+// Query i stands at position p = i + Tk - Tq and sees key s where
+//   s <= p  and  (s > p - window  or  s < sinks)  and  p, s < length of the sequence.
+//   P = exp(scale q.k - m) / l over the visible keys,  out = P v  (0 for a query without keys)
+//   D = dout . out,  dV = P^T dout,  dS = P (dout v^T - D),  dQ = scale dS K,  dK = scale dS^T Q
+// with dK and dV summed over the query heads of a KV head.
+#pragma once
+
+#include "fsi_common.h"
+
+namespace fsi_sink {
+
+constexpr int SK_T = 64;  // queries / keys per tile
+
+struct SkParams {
+  const void* q;
+  int64_t qs_b, qs_h, qs_t;
+  const void* k;
+  int64_t ks_b, ks_h, ks_t;
+  const void* v;
+  int64_t vs_b, vs_h, vs_t;
+  void* o;  // forward: written
+  int64_t os_b, os_h, os_t;
+  const void* dout;
+  int64_t ds_b, ds_h, ds_t;
+  int B, Hq, Hkv, Tq, Tk, hd, window, sinks;
+  const int32_t* lengths;
+  float scale;
+  float* lse;  // (B, Hq, Tq): log2 of the softmax denominator of scale log2(e) q.k; +inf without keys
+  float* dd;   // (B, Hq, Tq): D
+  void* dq;    // contiguous gradients of the operands' type
+  void* dk;
+  void* dv;
+};
+
+__device__ __forceinline__ int sk_length(const SkParams& P, int b) {
+  if (!P.lengths) return P.Tk;
+  const int n = P.lengths[b];
+  return n < 0 ? 0 : (n > P.Tk ? P.Tk : n);
+}
+
+// Key tiles that the queries at positions [p0, p1] reach: [0, n_sink) and [w0, w1].
+struct SkTiles {
+  int n_sink, w0, w1;
+  __device__ __forceinline__ int count() const { return n_sink + (w1 >= w0 ? w1 - w0 + 1 : 0); }
+  __device__ __forceinline__ int tile(int i) const { return i < n_sink ? i : w0 + i - n_sink; }
+};
+__device__ __forceinline__ SkTiles sk_key_tiles(const SkParams& P, int p0, int p1) {
+  SkTiles t;
+  if (p1 < p0) return {0, 0, -1};
+  const int wlo = p0 - P.window + 1 > 0 ? p0 - P.window + 1 : 0;  // first key of the first query's window
+  const int se = P.sinks < wlo ? P.sinks : wlo;                   // sinks before it
+  t.n_sink = (se + SK_T - 1) / SK_T;
+  t.w0 = wlo / SK_T > t.n_sink ? wlo / SK_T : t.n_sink;
+  t.w1 = P.window > 0 || P.sinks > wlo ? p1 / SK_T : -1;
+  return t;
+}
+
+__device__ __forceinline__ bool sk_visible(const SkParams& P, int len, int p, int s) {
+  return s <= p && (s > p - P.window || s < P.sinks) && p < len;
+}
+
+}  // namespace fsi_sink

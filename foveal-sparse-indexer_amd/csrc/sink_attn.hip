@@ -1,0 +1,395 @@
+// Attention over a sliding window and sinks (sink_attn.h): the C ABI, and the kernels for every
+// type, head size and alignment, on fp32 MFMA (v_mfma_f32_16x16x4_f32) over LDS tiles of 64 keys
+// (or queries) in fp32.  A wave owns 16 queries (or keys); a score tile's accumulators hold, per
+// lane, rows 4 kg + j of column r, and step j of the next product takes rows {4 kg + j} as its
+// four contraction indices, so P and dS enter it where they are.
+#include <algorithm>
+
+#include "sink_attn.h"
+
+using namespace fsi;
+using namespace fsi_sink;
+
+namespace {
+
+constexpr int SK_THREADS = 256;
+constexpr float SK_LOG2E = 1.4426950408889634f;
+
+template <typename T>
+__device__ __forceinline__ float sk_ld(const T* p, int64_t i);
+template <>
+__device__ __forceinline__ float sk_ld<float>(const float* p, int64_t i) { return p[i]; }
+template <>
+__device__ __forceinline__ float sk_ld<bf16_t>(const bf16_t* p, int64_t i) { return bf16_to_f32(p[i]); }
+__device__ __forceinline__ void sk_st(float* p, float x) { *p = x; }
+__device__ __forceinline__ void sk_st(bf16_t* p, float x) { *p = f32_to_bf16(x); }
+
+__device__ __forceinline__ f32x4_t mfma4(float a, float b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+// Rows [r0, r0 + 64) of a (n, hd) matrix into an LDS tile of row stride HD + 4 (the pad puts the
+// 16 rows of a column read on distinct banks); rows from n on and dims from hd on read as 0.
+template <typename T, int HD>
+__device__ __forceinline__ void sk_tile(const T* base, int64_t rs, int r0, int n, int hd, float* tile) {
+  for (int i = threadIdx.x; i < SK_T * HD; i += SK_THREADS) {
+    const int row = i / HD, d = i % HD;
+    tile[row * (HD + 4) + d] = r0 + row < n && d < hd ? sk_ld(base, (r0 + row) * rs + d) : 0.f;
+  }
+}
+
+// Row `row` of a (., hd) matrix as an operand: dims 4 s + kg; 0 where !ok.
+template <typename T, int HD>
+__device__ __forceinline__ void sk_frag(const T* base, int64_t rs, int row, bool ok, int hd, int kg, float (&f)[HD / 4]) {
+#pragma unroll
+  for (int s = 0; s < HD / 4; ++s) f[s] = ok && 4 * s + kg < hd ? sk_ld(base, row * rs + 4 * s + kg) : 0.f;
+}
+
+// X^T (16 rows of the tile from 16 t) against the wave's operand.
+template <int HD>
+__device__ __forceinline__ f32x4_t sk_scores(const float* tile, int t, int r, int kg, const float (&f)[HD / 4]) {
+  f32x4_t s = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const float* row = tile + (16 * t + r) * (HD + 4) + kg;
+#pragma unroll
+  for (int i = 0; i < HD / 4; ++i) s = mfma4(row[4 * i], f[i], s);
+  return s;
+}
+
+// acc[dim][col] += sum over the tile's rows X[row][dim] w[row][col]; w holds rows 16 t + 4 kg + j.
+template <int HD>
+__device__ __forceinline__ void sk_accumulate(const float* tile, int r, int kg, const f32x4_t (&w)[4],
+                                              f32x4_t (&acc)[HD / 16]) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float* row = tile + (16 * t + 4 * kg + j) * (HD + 4) + r;
+#pragma unroll
+      for (int dt = 0; dt < HD / 16; ++dt) acc[dt] = mfma4(row[16 * dt], w[t][j], acc[dt]);
+    }
+}
+
+// Column r of acc (dims 16 dt + 4 kg + j) times f into a row.
+template <typename T, int HD>
+__device__ __forceinline__ void sk_store(T* row, int hd, int kg, const f32x4_t (&acc)[HD / 16], float f) {
+#pragma unroll
+  for (int dt = 0; dt < HD / 16; ++dt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (16 * dt + 4 * kg + j < hd) sk_st(row + 16 * dt + 4 * kg + j, acc[dt][j] * f);
+}
+
+template <typename T, int HD>
+__global__ __launch_bounds__(SK_THREADS) void sk_fwd_kernel(SkParams P) {
+  extern __shared__ __attribute__((aligned(16))) float sk_smem[];
+  float *kt = sk_smem, *vt = sk_smem + SK_T * (HD + 4);
+  const int h = blockIdx.x % P.Hq, b = blockIdx.y, g = h / (P.Hq / P.Hkv);
+  const int i0 = (gridDim.x / P.Hq - 1 - blockIdx.x / P.Hq) * SK_T;  // most keys first
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kg = lane >> 4;
+  const int off = P.Tk - P.Tq, len = sk_length(P, b);
+  const int i = i0 + 16 * wave + r, p = off + i;
+  const bool live = i < P.Tq && p < len;
+  const T* k = static_cast<const T*>(P.k) + b * P.ks_b + g * P.ks_h;
+  const T* v = static_cast<const T*>(P.v) + b * P.vs_b + g * P.vs_h;
+  float qf[HD / 4];
+  sk_frag<T, HD>(static_cast<const T*>(P.q) + b * P.qs_b + h * P.qs_h, P.qs_t, i, live, P.hd, kg, qf);
+  f32x4_t acc[HD / 16];
+#pragma unroll
+  for (int dt = 0; dt < HD / 16; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  const float sl2 = P.scale * SK_LOG2E;
+  const SkTiles tiles = sk_key_tiles(P, off + i0, min(off + min(i0 + SK_T, P.Tq), len) - 1);
+  const int n = tiles.count();
+  for (int c = 0; c < n; ++c) {
+    const int s0 = tiles.tile(c) * SK_T;
+    __syncthreads();
+    sk_tile<T, HD>(k, P.ks_t, s0, len, P.hd, kt);
+    sk_tile<T, HD>(v, P.vs_t, s0, len, P.hd, vt);
+    __syncthreads();
+    f32x4_t st[4];
+    float mx = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      st[t] = sk_scores<HD>(kt, t, r, kg, qf);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        st[t][j] = live && sk_visible(P, len, p, s0 + 16 * t + 4 * kg + j) ? st[t][j] * sl2 : -INFINITY;
+        mx = fmaxf(mx, st[t][j]);
+      }
+    }
+    const float m_new = fmaxf(m, max_rows4(mx));
+    const float ref = m_new == -INFINITY ? 0.f : m_new;  // nothing visible yet: every p is 0
+    const float alpha = __builtin_amdgcn_exp2f(m - ref);
+    m = m_new;
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        st[t][j] = __builtin_amdgcn_exp2f(st[t][j] - ref);
+        sum += st[t][j];
+      }
+    l = l * alpha + sum_rows4(sum);
+#pragma unroll
+    for (int dt = 0; dt < HD / 16; ++dt) acc[dt] *= alpha;
+    sk_accumulate<HD>(vt, r, kg, st, acc);
+  }
+  if (i >= P.Tq) return;
+  sk_store<T, HD>(static_cast<T*>(P.o) + b * P.os_b + h * P.os_h + i * P.os_t, P.hd, kg, acc, l == 0.f ? 0.f : 1.f / l);
+  if (P.lse && kg == 0)
+    P.lse[(static_cast<int64_t>(b) * P.Hq + h) * P.Tq + i] = l == 0.f ? INFINITY : m + __log2f(l);
+}
+
+// dQ of 16 queries a wave, and D.
+template <typename T, int HD>
+__global__ __launch_bounds__(SK_THREADS) void sk_dq_kernel(SkParams P) {
+  extern __shared__ __attribute__((aligned(16))) float sk_smem[];
+  float *kt = sk_smem, *vt = sk_smem + SK_T * (HD + 4);
+  const int h = blockIdx.x % P.Hq, b = blockIdx.y, g = h / (P.Hq / P.Hkv);
+  const int i0 = (gridDim.x / P.Hq - 1 - blockIdx.x / P.Hq) * SK_T;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kg = lane >> 4;
+  const int off = P.Tk - P.Tq, len = sk_length(P, b);
+  const int i = i0 + 16 * wave + r, p = off + i;
+  const bool live = i < P.Tq && p < len;
+  const T* k = static_cast<const T*>(P.k) + b * P.ks_b + g * P.ks_h;
+  const T* v = static_cast<const T*>(P.v) + b * P.vs_b + g * P.vs_h;
+  const int64_t stat = (static_cast<int64_t>(b) * P.Hq + h) * P.Tq + i;
+  float qf[HD / 4], df[HD / 4];
+  sk_frag<T, HD>(static_cast<const T*>(P.q) + b * P.qs_b + h * P.qs_h, P.qs_t, i, live, P.hd, kg, qf);
+  sk_frag<T, HD>(static_cast<const T*>(P.dout) + b * P.ds_b + h * P.ds_h, P.ds_t, i, live, P.hd, kg, df);
+  const T* o = static_cast<const T*>(P.o) + b * P.os_b + h * P.os_h + i * P.os_t;
+  float dd = 0.f;
+#pragma unroll
+  for (int s = 0; s < HD / 4; ++s)
+    if (live && 4 * s + kg < P.hd) dd = fmaf(df[s], sk_ld(o, 4 * s + kg), dd);
+  dd = sum_rows4(dd);
+  if (i < P.Tq && kg == 0) P.dd[stat] = dd;
+  const float lse = live ? P.lse[stat] : INFINITY, sl2 = P.scale * SK_LOG2E;
+  f32x4_t acc[HD / 16];
+#pragma unroll
+  for (int dt = 0; dt < HD / 16; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const SkTiles tiles = sk_key_tiles(P, off + i0, min(off + min(i0 + SK_T, P.Tq), len) - 1);
+  const int n = tiles.count();
+  for (int c = 0; c < n; ++c) {
+    const int s0 = tiles.tile(c) * SK_T;
+    __syncthreads();
+    sk_tile<T, HD>(k, P.ks_t, s0, len, P.hd, kt);
+    sk_tile<T, HD>(v, P.vs_t, s0, len, P.hd, vt);
+    __syncthreads();
+    f32x4_t ds[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const f32x4_t s = sk_scores<HD>(kt, t, r, kg, qf), dp = sk_scores<HD>(vt, t, r, kg, df);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool ok = live && sk_visible(P, len, p, s0 + 16 * t + 4 * kg + j);
+        ds[t][j] = ok ? __builtin_amdgcn_exp2f(fmaf(s[j], sl2, -lse)) * (dp[j] - dd) : 0.f;
+      }
+    }
+    sk_accumulate<HD>(kt, r, kg, ds, acc);
+  }
+  if (i < P.Tq)
+    sk_store<T, HD>(static_cast<T*>(P.dq) + ((static_cast<int64_t>(b) * P.Hq + h) * P.Tq + i) * P.hd, P.hd, kg, acc,
+                    P.scale);
+}
+
+// dK and dV of 16 keys a wave: every query tile that reaches the 64 keys, every query head.
+template <typename T, int HD>
+__global__ __launch_bounds__(SK_THREADS, 1) void sk_dkv_kernel(SkParams P) {
+  extern __shared__ __attribute__((aligned(16))) float sk_smem[];
+  float *qt = sk_smem, *gt = sk_smem + SK_T * (HD + 4), *stats = sk_smem + 2 * SK_T * (HD + 4);
+  const int g = blockIdx.x % P.Hkv, b = blockIdx.y, s0 = static_cast<int>(blockIdx.x / P.Hkv) * SK_T;
+  const int G = P.Hq / P.Hkv;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kg = lane >> 4;
+  const int off = P.Tk - P.Tq, len = sk_length(P, b);
+  const int s = s0 + 16 * wave + r;
+  float kf[HD / 4], vf[HD / 4];
+  sk_frag<T, HD>(static_cast<const T*>(P.k) + b * P.ks_b + g * P.ks_h, P.ks_t, s, s < len, P.hd, kg, kf);
+  sk_frag<T, HD>(static_cast<const T*>(P.v) + b * P.vs_b + g * P.vs_h, P.vs_t, s, s < len, P.hd, kg, vf);
+  f32x4_t dk[HD / 16], dv[HD / 16];
+#pragma unroll
+  for (int dt = 0; dt < HD / 16; ++dt) dk[dt] = dv[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const float sl2 = P.scale * SK_LOG2E;
+  // queries at positions [s0, s0 + 63 + window), or all from s0 on where sinks are among the keys
+  const int q_end = min(P.Tq, len - off);
+  const int64_t w_end = s0 < P.sinks ? q_end : static_cast<int64_t>(s0) + SK_T - 1 + P.window - off;
+  const int i_lo = max(0, s0 - off) / SK_T * SK_T, i_hi = w_end < q_end ? static_cast<int>(w_end) : q_end;
+  for (int i0 = i_lo; i0 < i_hi; i0 += SK_T)
+    for (int hh = 0; hh < G; ++hh) {
+      const int h = g * G + hh;
+      __syncthreads();
+      sk_tile<T, HD>(static_cast<const T*>(P.q) + b * P.qs_b + h * P.qs_h, P.qs_t, i0, q_end, P.hd, qt);
+      sk_tile<T, HD>(static_cast<const T*>(P.dout) + b * P.ds_b + h * P.ds_h, P.ds_t, i0, q_end, P.hd, gt);
+      if (threadIdx.x < 2 * SK_T) {
+        const int i = i0 + (threadIdx.x & 63);
+        const float* src = threadIdx.x < SK_T ? P.lse : P.dd;
+        stats[threadIdx.x] = i < q_end ? src[(static_cast<int64_t>(b) * P.Hq + h) * P.Tq + i] : 0.f;
+      }
+      __syncthreads();
+      f32x4_t pw[4], ds[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const f32x4_t sc = sk_scores<HD>(qt, t, r, kg, kf), dp = sk_scores<HD>(gt, t, r, kg, vf);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int row = 16 * t + 4 * kg + j, i = i0 + row;
+          const bool ok = i < q_end && sk_visible(P, len, off + i, s);
+          pw[t][j] = ok ? __builtin_amdgcn_exp2f(fmaf(sc[j], sl2, -stats[row])) : 0.f;
+          ds[t][j] = ok ? pw[t][j] * (dp[j] - stats[SK_T + row]) : 0.f;
+        }
+      }
+      sk_accumulate<HD>(gt, r, kg, pw, dv);
+      sk_accumulate<HD>(qt, r, kg, ds, dk);
+    }
+  if (s < P.Tk) {
+    const int64_t row = ((static_cast<int64_t>(b) * P.Hkv + g) * P.Tk + s) * P.hd;
+    sk_store<T, HD>(static_cast<T*>(P.dk) + row, P.hd, kg, dk, P.scale);
+    sk_store<T, HD>(static_cast<T*>(P.dv) + row, P.hd, kg, dv, 1.f);
+  }
+}
+
+// LDS above 64 KiB a workgroup has to be asked for.
+template <typename K>
+void sk_launch(K* kern, dim3 grid, size_t lds, hipStream_t st, const SkParams& P) {
+  if (lds > 65536)
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
+                              static_cast<int>(lds));
+  kern<<<grid, SK_THREADS, lds, st>>>(P);
+}
+
+template <typename F>
+void sk_by_width(int64_t hd, F&& f) {
+  if (hd <= 32) f(std::integral_constant<int, 32>{});
+  else if (hd <= 64) f(std::integral_constant<int, 64>{});
+  else if (hd <= 96) f(std::integral_constant<int, 96>{});
+  else if (hd <= 128) f(std::integral_constant<int, 128>{});
+  else f(std::integral_constant<int, 256>{});
+}
+
+int sk_check(const char* what, int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t hd, int64_t window,
+             int64_t sinks, int dtype) {
+  FSI_CHECK_ARG(dtype == FSI_DTYPE_F32 || dtype == FSI_DTYPE_BF16, FSI_ERR_DTYPE, "%s: dtype %d", what, dtype);
+  FSI_CHECK_ARG(hd >= 1 && hd <= 256, FSI_ERR_SHAPE, "%s: head_dim %lld (1..256)", what, (long long)hd);
+  FSI_CHECK_ARG(B >= 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Tq >= 0 && Tk >= Tq, FSI_ERR_SHAPE,
+                "%s: B %lld, Hq %lld, Hkv %lld, Tq %lld, Tk %lld (Hkv divides Hq, Tq <= Tk)", what, (long long)B,
+                (long long)Hq, (long long)Hkv, (long long)Tq, (long long)Tk);
+  FSI_CHECK_ARG(window >= 0 && sinks >= 0, FSI_ERR_SHAPE, "%s: window %lld, sinks %lld", what, (long long)window,
+                (long long)sinks);
+  FSI_CHECK_ARG(Tk <= (int64_t(1) << 30) && B <= 65535 && (Tk + SK_T - 1) / SK_T * Hq <= 0x7fffffff, FSI_ERR_SHAPE,
+                "%s: sizes beyond range", what);
+  return FSI_OK;
+}
+
+SkParams sk_params(const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_t, const void* k, int64_t ks_b, int64_t ks_h,
+                   int64_t ks_t, const void* v, int64_t vs_b, int64_t vs_h, int64_t vs_t, const void* o, int64_t os_b,
+                   int64_t os_h, int64_t os_t, int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t hd,
+                   int64_t window, int64_t sinks, const int32_t* lengths, float scale) {
+  SkParams P{};
+  P.q = q;
+  P.qs_b = qs_b;
+  P.qs_h = qs_h;
+  P.qs_t = qs_t;
+  P.k = k;
+  P.ks_b = ks_b;
+  P.ks_h = ks_h;
+  P.ks_t = ks_t;
+  P.v = v;
+  P.vs_b = vs_b;
+  P.vs_h = vs_h;
+  P.vs_t = vs_t;
+  P.o = const_cast<void*>(o);
+  P.os_b = os_b;
+  P.os_h = os_h;
+  P.os_t = os_t;
+  P.B = (int)B;
+  P.Hq = (int)Hq;
+  P.Hkv = (int)Hkv;
+  P.Tq = (int)Tq;
+  P.Tk = (int)Tk;
+  P.hd = (int)hd;
+  // a window or sinks past the sequence see all of it
+  P.window = (int)std::min<int64_t>(window, Tk);
+  P.sinks = (int)std::min<int64_t>(sinks, Tk);
+  P.lengths = lengths;
+  P.scale = scale;
+  return P;
+}
+
+}  // namespace
+
+extern "C" {
+
+FSI_API int fsi_sink_attn(const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_t, const void* k, int64_t ks_b,
+                          int64_t ks_h, int64_t ks_t, const void* v, int64_t vs_b, int64_t vs_h, int64_t vs_t,
+                          int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t head_dim, int64_t window,
+                          int64_t sinks, const int32_t* lengths, float scale, int dtype, void* out, int64_t os_b,
+                          int64_t os_h, int64_t os_t, float* lse, void* stream) {
+  const int c = sk_check("sink_attn", B, Hq, Hkv, Tq, Tk, head_dim, window, sinks, dtype);
+  if (c != FSI_OK || B == 0 || Tq == 0) return c;
+  FSI_CHECK_ARG(q && k && v && out, FSI_ERR_INVALID_ARG, "sink_attn: null pointer");
+  SkParams P = sk_params(q, qs_b, qs_h, qs_t, k, ks_b, ks_h, ks_t, v, vs_b, vs_h, vs_t, out, os_b, os_h, os_t, B, Hq,
+                         Hkv, Tq, Tk, head_dim, window, sinks, lengths, scale);
+  P.lse = lse;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const dim3 grid(static_cast<unsigned>((Tq + SK_T - 1) / SK_T * Hq), static_cast<unsigned>(B));
+  sk_by_width(head_dim, [&](auto w) {
+    constexpr int HD = decltype(w)::value;
+    const size_t lds = sizeof(float) * 2 * SK_T * (HD + 4);
+    if (dtype == FSI_DTYPE_F32) sk_launch(&sk_fwd_kernel<float, HD>, grid, lds, st, P);
+    else sk_launch(&sk_fwd_kernel<bf16_t, HD>, grid, lds, st, P);
+  });
+  FSI_HIP_LAUNCH_CHECK("sink_attn");
+  return FSI_OK;
+}
+
+FSI_API size_t fsi_sink_attn_bwd_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t Tk,
+                                                int64_t head_dim, int64_t window, int64_t sinks) {
+  (void)Hkv, (void)Tk, (void)head_dim, (void)window, (void)sinks;
+  if (B <= 0 || Hq <= 0 || Tq <= 0) return 0;
+  return sizeof(float) * static_cast<size_t>(B * Hq * Tq);
+}
+
+FSI_API int fsi_sink_attn_bwd(const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_t, const void* k, int64_t ks_b,
+                              int64_t ks_h, int64_t ks_t, const void* v, int64_t vs_b, int64_t vs_h, int64_t vs_t,
+                              const void* out, int64_t os_b, int64_t os_h, int64_t os_t, const void* dout, int64_t ds_b,
+                              int64_t ds_h, int64_t ds_t, const float* lse, int64_t B, int64_t Hq, int64_t Hkv,
+                              int64_t Tq, int64_t Tk, int64_t head_dim, int64_t window, int64_t sinks,
+                              const int32_t* lengths, float scale, int dtype, void* dq, void* dk, void* dv,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+  const int c = sk_check("sink_attn_bwd", B, Hq, Hkv, Tq, Tk, head_dim, window, sinks, dtype);
+  if (c != FSI_OK || B == 0 || Tk == 0) return c;
+  FSI_CHECK_ARG(dk && dv && (Tq == 0 || (q && k && v && out && dout && lse && dq)), FSI_ERR_INVALID_ARG,
+                "sink_attn_bwd: null pointer");
+  const size_t need = fsi_sink_attn_bwd_workspace_size(B, Hq, Hkv, Tq, Tk, head_dim, window, sinks);
+  FSI_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+                FSI_ERR_WORKSPACE, "sink_attn_bwd: workspace %zu < %zu bytes (or misaligned)", workspace_bytes, need);
+  SkParams P = sk_params(q, qs_b, qs_h, qs_t, k, ks_b, ks_h, ks_t, v, vs_b, vs_h, vs_t, out, os_b, os_h, os_t, B, Hq,
+                         Hkv, Tq, Tk, head_dim, window, sinks, lengths, scale);
+  P.dout = dout;
+  P.ds_b = ds_b;
+  P.ds_h = ds_h;
+  P.ds_t = ds_t;
+  P.lse = const_cast<float*>(lse);
+  P.dd = static_cast<float*>(workspace);
+  P.dq = dq;
+  P.dk = dk;
+  P.dv = dv;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const dim3 gq(static_cast<unsigned>((Tq + SK_T - 1) / SK_T * Hq), static_cast<unsigned>(B));
+  const dim3 gkv(static_cast<unsigned>((Tk + SK_T - 1) / SK_T * Hkv), static_cast<unsigned>(B));
+  sk_by_width(head_dim, [&](auto w) {
+    constexpr int HD = decltype(w)::value;
+    const size_t lds = sizeof(float) * 2 * SK_T * (HD + 4), lds_kv = lds + sizeof(float) * 2 * SK_T;
+    if (dtype == FSI_DTYPE_F32) {
+      if (Tq > 0) sk_launch(&sk_dq_kernel<float, HD>, gq, lds, st, P);
+      sk_launch(&sk_dkv_kernel<float, HD>, gkv, lds_kv, st, P);
+    } else {
+      if (Tq > 0) sk_launch(&sk_dq_kernel<bf16_t, HD>, gq, lds, st, P);
+      sk_launch(&sk_dkv_kernel<bf16_t, HD>, gkv, lds_kv, st, P);
+    }
+  });
+  FSI_HIP_LAUNCH_CHECK("sink_attn_bwd");
+  return FSI_OK;
+}
+
+}  // extern "C"

@@ -50,6 +50,9 @@ typedef enum fsi_status {
  * (fsi_sram_indexer_attention). */
 typedef enum fsi_dtype { FSI_DTYPE_F32 = 0, FSI_DTYPE_BF16 = 1, FSI_DTYPE_F16 = 2 } fsi_dtype;
 
+/* How a paged K/V pool holds its elements (fsi_kv_mx_*, fsi_decode_attn_sinks). */
+typedef enum fsi_kv_format { FSI_KV_BF16 = 0, FSI_KV_MXFP8 = 1, FSI_KV_MXFP4 = 2 } fsi_kv_format;
+
 /* Size of the zero-initialised arrival-counter area at the start of every workspace. */
 #define FSI_WORKSPACE_COUNTER_BYTES 65536
 
@@ -534,6 +537,57 @@ FSI_API int fsi_decode_attn_bwd_q(const void* q, const void* dout, const void* k
                                   float* dq, int* err, void* stream);
 
 /* ------------------------------------------------------------------------- *
+ * Paged pools held in 8 or 4 bits, and decode attention with sinks.  No counterpart
+ * in the reference, whose cache holds the model's type (attention.py:45-57).
+ *
+ * 32 consecutive dims of one token and KV head share a power of two: element = value
+ * 2^e with e4m3 (FSI_KV_MXFP8) or e2m1 (FSI_KV_MXFP4) values and the scale byte e + 127.
+ * e is the smallest integer with max|x| <= 464 2^e (7 2^e), kept in [-116, 119]
+ * ([-116, 125]); x 2^-e is rounded to the nearest value, ties to even, clamped to
+ * +-448 (+-6).  A group with an infinity or a NaN reads back as NaN.
+ * head_dim 64, 96, 128 or 256; pages of 64 tokens.  The pools are arrays of
+ * fsi_kv_mx_block_bytes(head_dim, format) bytes per (physical page, KV head), for K
+ * and for V (csrc/mx_cache.h has the layout); 0 for sizes that are not supported.
+ * ------------------------------------------------------------------------- */
+FSI_API int64_t fsi_kv_mx_block_bytes(int64_t head_dim, int format);
+
+/* Write n_tok tokens per sequence at positions start_rows[b] (or start) .. as
+ * fsi_kv_write does, from K and V of dtype (FSI_DTYPE_BF16 or FSI_DTYPE_F32) with any
+ * element strides over (B, Hkv, n_tok) and unit stride over head_dim.  Positions outside
+ * the page table and pages outside the pool are skipped and reported through err. */
+FSI_API int fsi_kv_mx_write(const void* k, const void* v, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_t,
+                            int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_t, int64_t B, int64_t Hkv,
+                            int64_t n_tok, int64_t head_dim, int dtype, int format, const int32_t* start_rows,
+                            int64_t start, const int32_t* page_table, int64_t max_pages, int64_t n_phys_pages,
+                            void* k_pool, void* v_pool, int* err, void* stream);
+
+/* Read tokens [0, n_tok) of every sequence back to contiguous (B, Hkv, n_tok, head_dim)
+ * K and V of dtype: exactly the values held.  Tokens without a page read as 0. */
+FSI_API int fsi_kv_mx_read(const void* k_pool, const void* v_pool, int format, int64_t B, int64_t Hkv, int64_t n_tok,
+                           int64_t head_dim, const int32_t* page_table, int64_t max_pages, int64_t n_phys_pages,
+                           int dtype, void* k_out, void* v_out, void* stream);
+
+/* Decode attention over pools of any fsi_kv_format, with sinks: out (B, Hq, head_dim) =
+ * softmax(scale q K^T) V over, with ls = max(0, pos + 1 - window) and se = min(sinks, ls),
+ *   tokens [0, se), tokens [ls, pos], and the tokens in [se, ls) of the pages
+ *   remote_pages[b, :remote_counts[b]]
+ * (a token of several of these counts once; a page listed twice counts twice).  A sequence
+ * without any token gets 0.  q and out contiguous, of dtype: FSI_DTYPE_BF16, or
+ * FSI_DTYPE_F32 with the 8- and 4-bit formats (an fp32 result).  head_dim 64 or 128 for
+ * FSI_KV_BF16 (the pools of fsi_kv_write), else 64, 96, 128 or 256; any Hq / Hkv.  Pages
+ * outside the table or the pool are skipped and reported through err.  Workspace: partial
+ * results, written before they are read (need not be zeroed), 16-byte aligned. */
+FSI_API size_t fsi_decode_attn_sinks_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t head_dim, int format,
+                                                    int64_t window, int64_t sinks, int64_t capacity,
+                                                    int64_t max_pages);
+FSI_API int fsi_decode_attn_sinks(const void* q, int dtype, const void* k_pool, const void* v_pool, int format,
+                                  const int32_t* page_table, int64_t max_pages, int64_t n_phys_pages,
+                                  const int32_t* pos_rows, int64_t pos, int64_t window, int64_t sinks,
+                                  const int32_t* remote_pages, const int32_t* remote_counts, int64_t capacity,
+                                  int64_t B, int64_t Hq, int64_t Hkv, int64_t head_dim, float scale, void* out,
+                                  void* workspace, size_t workspace_bytes, int* err, void* stream);
+
+/* ------------------------------------------------------------------------- *
  * Block-sparse prefill attention (bf16 in, fp32 softmax and accumulate, bf16 out).
  * q: (B, Hq, T, head_dim), k and v: (B, Hkv, T, head_dim), out: (B, Hq, T,
  * head_dim), each given by element strides (s_b, s_h, s_t; unit stride over
@@ -591,6 +645,40 @@ FSI_API int fsi_sparse_attn_bwd(const void* q, int64_t qs_b, int64_t qs_h, int64
                                 const int32_t* counts, int64_t cs_b, int64_t cs_q, float scale, int dtype, float* dq,
                                 float* dk, float* dv, void* workspace, size_t workspace_bytes, int* err,
                                 void* stream);
+
+/* ------------------------------------------------------------------------- *
+ * Attention over a sliding window and the first tokens ("sinks"), forward and backward.
+ * No counterpart in the reference (its local window is always joined by routed pages,
+ * attention.py:148-178).  q and out (B, Hq, Tq, head_dim), k and v (B, Hkv, Tk, head_dim),
+ * Tq <= Tk: query i stands at position p = i + Tk - Tq and sees key s where s <= p, and
+ * s > p - window or s < sinks, and p and s are below lengths[b] (null: Tk).  A query that
+ * sees no key gets 0; the memory behind a sequence's length is not used.  Query head h
+ * uses KV head h / (Hq / Hkv).  Element strides over (B, H, T), unit stride over
+ * head_dim 1..256; dtype FSI_DTYPE_BF16 or FSI_DTYPE_F32, fp32 softmax and sums.  bf16 with
+ * head_dim 64 or 128, 16-byte aligned pointers and strides of multiples of 8 elements
+ * runs on bf16 MFMA, everything else on fp32 MFMA.
+ * lse (B, Hq, Tq) fp32 (null: not wanted): log2 of each query's softmax denominator in
+ * units of scale log2(e) q.k, which the backward takes; +inf for a query without keys.
+ *
+ * The backward writes contiguous dq (B, Hq, Tq, head_dim), dk and dv (B, Hkv, Tk, head_dim)
+ * of dtype, dk and dv summed over the query heads of a KV head in fp32, in a fixed order.
+ * Workspace: written before it is read (need not be zeroed), 16-byte aligned.
+ * ------------------------------------------------------------------------- */
+FSI_API int fsi_sink_attn(const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_t, const void* k, int64_t ks_b,
+                          int64_t ks_h, int64_t ks_t, const void* v, int64_t vs_b, int64_t vs_h, int64_t vs_t,
+                          int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t head_dim, int64_t window,
+                          int64_t sinks, const int32_t* lengths, float scale, int dtype, void* out, int64_t os_b,
+                          int64_t os_h, int64_t os_t, float* lse, void* stream);
+
+FSI_API size_t fsi_sink_attn_bwd_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t Tk,
+                                                int64_t head_dim, int64_t window, int64_t sinks);
+FSI_API int fsi_sink_attn_bwd(const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_t, const void* k, int64_t ks_b,
+                              int64_t ks_h, int64_t ks_t, const void* v, int64_t vs_b, int64_t vs_h, int64_t vs_t,
+                              const void* out, int64_t os_b, int64_t os_h, int64_t os_t, const void* dout, int64_t ds_b,
+                              int64_t ds_h, int64_t ds_t, const float* lse, int64_t B, int64_t Hq, int64_t Hkv,
+                              int64_t Tq, int64_t Tk, int64_t head_dim, int64_t window, int64_t sinks,
+                              const int32_t* lengths, float scale, int dtype, void* dq, void* dk, void* dv,
+                              void* workspace, size_t workspace_bytes, void* stream);
 
 /* Fused 16-D block indexer + greedy block selection + block attention
  * (triton_fused_sram_indexer_attention, foveal_indexer/triton_ops.py:142-249,373-435).
