@@ -62,4 +62,27 @@ __device__ __forceinline__ bool sk_visible(const SkParams& P, int len, int p, in
   return s <= p && (s > p - P.window || s < P.sinks) && p < len;
 }
 
+// A tile of sink keys is seen by every later query, far more than a window's: its queries beyond
+// the window are cut into `parts` of `span` queries (a multiple of the tile), each a workgroup of
+// its own that leaves fp32 sums of the sink rows in `sums` (B, Hkv, parts + 1, sinks, [dK, dV], hd),
+// the window's own queries as the last part; sk_sink_sum_kernel adds them in that order.
+// parts 0: no such split, a sink tile's workgroup takes all of its queries.
+struct SkSinkSplit {
+  int tiles, parts, span;
+  float* sums;
+};
+
+// End of the queries that reach key tile s0 before the split's parts begin, in whole query tiles.
+__device__ __forceinline__ int sk_near_end(const SkParams& P, const SkSinkSplit& S, int s0) {
+  if (s0 < P.sinks && S.parts == 0) return P.Tq;
+  const int64_t end = static_cast<int64_t>(s0) + SK_T - 1 + P.window - (P.Tk - P.Tq);
+  if (end <= 0) return 0;
+  return static_cast<int>(end < P.Tq ? (end + SK_T - 1) / SK_T * SK_T : P.Tq);
+}
+
+// The bf16 kernels of sink_attn_bf16.hip: whether they take the call, and their launches.
+bool sb_takes(const SkParams& P, int dtype, bool backward);
+void sb_forward(const SkParams& P, hipStream_t st);
+void sb_backward(const SkParams& P, const SkSinkSplit& S, hipStream_t st);
+
 }  // namespace fsi_sink

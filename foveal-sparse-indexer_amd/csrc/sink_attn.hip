@@ -195,11 +195,14 @@ __global__ __launch_bounds__(SK_THREADS) void sk_dq_kernel(SkParams P) {
 
 // dK and dV of 16 keys a wave: every query tile that reaches the 64 keys, every query head.
 template <typename T, int HD>
-__global__ __launch_bounds__(SK_THREADS, 1) void sk_dkv_kernel(SkParams P) {
+__global__ __launch_bounds__(SK_THREADS, 1) void sk_dkv_kernel(SkParams P, SkSinkSplit S) {
   extern __shared__ __attribute__((aligned(16))) float sk_smem[];
   float *qt = sk_smem, *gt = sk_smem + SK_T * (HD + 4), *stats = sk_smem + 2 * SK_T * (HD + 4);
-  const int g = blockIdx.x % P.Hkv, b = blockIdx.y, s0 = static_cast<int>(blockIdx.x / P.Hkv) * SK_T;
-  const int G = P.Hq / P.Hkv;
+  const int g = static_cast<int>(blockIdx.x) % P.Hkv, b = blockIdx.y;
+  // the parts of the split sink tiles come first: they are the longest
+  const int x = static_cast<int>(blockIdx.x) / P.Hkv, n_far = S.tiles * S.parts;
+  const int tile = x < n_far ? x / S.parts : x - n_far, part = x < n_far ? x % S.parts : -1;
+  const int s0 = tile * SK_T, G = P.Hq / P.Hkv;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kg = lane >> 4;
   const int off = P.Tk - P.Tq, len = sk_length(P, b);
   const int s = s0 + 16 * wave + r;
@@ -210,10 +213,10 @@ __global__ __launch_bounds__(SK_THREADS, 1) void sk_dkv_kernel(SkParams P) {
 #pragma unroll
   for (int dt = 0; dt < HD / 16; ++dt) dk[dt] = dv[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   const float sl2 = P.scale * SK_LOG2E;
-  // queries at positions [s0, s0 + 63 + window), or all from s0 on where sinks are among the keys
-  const int q_end = min(P.Tq, len - off);
-  const int64_t w_end = s0 < P.sinks ? q_end : static_cast<int64_t>(s0) + SK_T - 1 + P.window - off;
-  const int i_lo = max(0, s0 - off) / SK_T * SK_T, i_hi = w_end < q_end ? static_cast<int>(w_end) : q_end;
+  // queries that reach the keys through the window, or the part's beyond it
+  const int q_end = min(P.Tq, len - off), near_hi = sk_near_end(P, S, s0);
+  const int i_lo = part < 0 ? max(0, s0 - off) / SK_T * SK_T : near_hi + part * S.span;
+  const int i_hi = min(q_end, part < 0 ? near_hi : i_lo + S.span);
   for (int i0 = i_lo; i0 < i_hi; i0 += SK_T)
     for (int hh = 0; hh < G; ++hh) {
       const int h = g * G + hh;
@@ -241,20 +244,56 @@ __global__ __launch_bounds__(SK_THREADS, 1) void sk_dkv_kernel(SkParams P) {
       sk_accumulate<HD>(gt, r, kg, pw, dv);
       sk_accumulate<HD>(qt, r, kg, ds, dk);
     }
-  if (s < P.Tk) {
-    const int64_t row = ((static_cast<int64_t>(b) * P.Hkv + g) * P.Tk + s) * P.hd;
+  if (s >= P.Tk) return;
+  const int64_t head = static_cast<int64_t>(b) * P.Hkv + g;
+  if (n_far > 0 && s < P.sinks) {  // a term of the row's sum
+    float* t = S.sums + (((head * (S.parts + 1) + (part < 0 ? S.parts : part)) * P.sinks + s) * 2) * P.hd;
+    sk_store<float, HD>(t, P.hd, kg, dk, P.scale);
+    sk_store<float, HD>(t + P.hd, P.hd, kg, dv, 1.f);
+  } else if (part < 0) {
+    const int64_t row = (head * P.Tk + s) * P.hd;
     sk_store<T, HD>(static_cast<T*>(P.dk) + row, P.hd, kg, dk, P.scale);
     sk_store<T, HD>(static_cast<T*>(P.dv) + row, P.hd, kg, dv, 1.f);
   }
 }
 
+// dK and dV rows of split sink tiles: the parts' sums in order, one workgroup per (head, sink).
+template <typename T>
+__global__ __launch_bounds__(SK_THREADS) void sk_sink_sum_kernel(SkParams P, SkSinkSplit S) {
+  const int s = static_cast<int>(blockIdx.x) % P.sinks;
+  const int64_t head = blockIdx.x / P.sinks;
+  for (int d = threadIdx.x; d < 2 * P.hd; d += SK_THREADS) {
+    float sum = 0.f;
+    for (int part = 0; part <= S.parts; ++part)
+      sum += S.sums[((head * (S.parts + 1) + part) * P.sinks + s) * 2 * P.hd + d];
+    T* out = static_cast<T*>(d < P.hd ? P.dk : P.dv) + (head * P.Tk + s) * P.hd + (d < P.hd ? d : d - P.hd);
+    sk_st(out, sum);
+  }
+}
+
+// A part has about a window tile's queries, and no fewer than 512 (a short part's start and sum
+// cost more than it saves).  More than 1024 sinks are tiles enough to fill the chip by themselves.
+SkSinkSplit sk_split(int64_t Tq, int64_t Tk, int64_t window, int64_t sinks) {
+  SkSinkSplit S{};
+  window = std::min(window, Tk);
+  sinks = std::min(sinks, Tk);
+  if (sinks <= 0 || sinks > 1024) return S;
+  const int64_t span = std::max<int64_t>(512, (window + 2 * SK_T - 1) / SK_T * SK_T);
+  const int64_t near_hi = std::max<int64_t>((SK_T - 1 + window - (Tk - Tq) + SK_T - 1) / SK_T * SK_T, 0);
+  if (Tq - near_hi <= span) return S;
+  S.tiles = static_cast<int>((sinks + SK_T - 1) / SK_T);
+  S.parts = static_cast<int>((Tq - near_hi + span - 1) / span);
+  S.span = static_cast<int>(span);
+  return S;
+}
+
 // LDS above 64 KiB a workgroup has to be asked for.
-template <typename K>
-void sk_launch(K* kern, dim3 grid, size_t lds, hipStream_t st, const SkParams& P) {
+template <typename K, typename... A>
+void sk_launch(K* kern, dim3 grid, size_t lds, hipStream_t st, const A&... args) {
   if (lds > 65536)
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
                               static_cast<int>(lds));
-  kern<<<grid, SK_THREADS, lds, st>>>(P);
+  kern<<<grid, SK_THREADS, lds, st>>>(args...);
 }
 
 template <typename F>
@@ -331,6 +370,11 @@ FSI_API int fsi_sink_attn(const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_
                          Hkv, Tq, Tk, head_dim, window, sinks, lengths, scale);
   P.lse = lse;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (sb_takes(P, dtype, false)) {
+    sb_forward(P, st);
+    FSI_HIP_LAUNCH_CHECK("sink_attn");
+    return FSI_OK;
+  }
   const dim3 grid(static_cast<unsigned>((Tq + SK_T - 1) / SK_T * Hq), static_cast<unsigned>(B));
   sk_by_width(head_dim, [&](auto w) {
     constexpr int HD = decltype(w)::value;
@@ -344,9 +388,11 @@ FSI_API int fsi_sink_attn(const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_
 
 FSI_API size_t fsi_sink_attn_bwd_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t Tk,
                                                 int64_t head_dim, int64_t window, int64_t sinks) {
-  (void)Hkv, (void)Tk, (void)head_dim, (void)window, (void)sinks;
-  if (B <= 0 || Hq <= 0 || Tq <= 0) return 0;
-  return sizeof(float) * static_cast<size_t>(B * Hq * Tq);
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Tq <= 0 || Tk < Tq || head_dim <= 0 || window < 0 || sinks < 0) return 0;
+  const SkSinkSplit S = sk_split(Tq, Tk, window, sinks);
+  // D of every query, then the split sink tiles' sums
+  return fsi_host::align_up(sizeof(float) * static_cast<size_t>(B * Hq * Tq), 256) +
+         (S.parts ? sizeof(float) * static_cast<size_t>(B * Hkv * (S.parts + 1) * std::min(sinks, Tk) * 2 * head_dim) : 0);
 }
 
 FSI_API int fsi_sink_attn_bwd(const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_t, const void* k, int64_t ks_b,
@@ -356,6 +402,7 @@ FSI_API int fsi_sink_attn_bwd(const void* q, int64_t qs_b, int64_t qs_h, int64_t
                               int64_t Tq, int64_t Tk, int64_t head_dim, int64_t window, int64_t sinks,
                               const int32_t* lengths, float scale, int dtype, void* dq, void* dk, void* dv,
                               void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace fsi_host;
   const int c = sk_check("sink_attn_bwd", B, Hq, Hkv, Tq, Tk, head_dim, window, sinks, dtype);
   if (c != FSI_OK || B == 0 || Tk == 0) return c;
   FSI_CHECK_ARG(dk && dv && (Tq == 0 || (q && k && v && out && dout && lse && dq)), FSI_ERR_INVALID_ARG,
@@ -375,19 +422,38 @@ FSI_API int fsi_sink_attn_bwd(const void* q, int64_t qs_b, int64_t qs_h, int64_t
   P.dk = dk;
   P.dv = dv;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  SkSinkSplit S = sk_split(Tq, Tk, window, sinks);
+  FSI_CHECK_ARG(B * Hkv * P.sinks <= 0x7fffffff && ((Tk + SK_T - 1) / SK_T + S.tiles * S.parts) * Hkv <= 0x7fffffff,
+                FSI_ERR_SHAPE, "sink_attn_bwd: sizes beyond range");
+  if (S.parts)
+    S.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                      align_up(sizeof(float) * static_cast<size_t>(B * Hq * Tq), 256));
+  auto sum_sinks = [&] {
+    if (!S.parts) return;
+    const unsigned rows = static_cast<unsigned>(B * Hkv * P.sinks);
+    if (dtype == FSI_DTYPE_F32) sk_sink_sum_kernel<float><<<rows, SK_THREADS, 0, st>>>(P, S);
+    else sk_sink_sum_kernel<bf16_t><<<rows, SK_THREADS, 0, st>>>(P, S);
+  };
+  if (sb_takes(P, dtype, true)) {
+    sb_backward(P, S, st);
+    sum_sinks();
+    FSI_HIP_LAUNCH_CHECK("sink_attn_bwd");
+    return FSI_OK;
+  }
   const dim3 gq(static_cast<unsigned>((Tq + SK_T - 1) / SK_T * Hq), static_cast<unsigned>(B));
-  const dim3 gkv(static_cast<unsigned>((Tk + SK_T - 1) / SK_T * Hkv), static_cast<unsigned>(B));
+  const dim3 gkv(static_cast<unsigned>(((Tk + SK_T - 1) / SK_T + S.tiles * S.parts) * Hkv), static_cast<unsigned>(B));
   sk_by_width(head_dim, [&](auto w) {
     constexpr int HD = decltype(w)::value;
     const size_t lds = sizeof(float) * 2 * SK_T * (HD + 4), lds_kv = lds + sizeof(float) * 2 * SK_T;
     if (dtype == FSI_DTYPE_F32) {
       if (Tq > 0) sk_launch(&sk_dq_kernel<float, HD>, gq, lds, st, P);
-      sk_launch(&sk_dkv_kernel<float, HD>, gkv, lds_kv, st, P);
+      sk_launch(&sk_dkv_kernel<float, HD>, gkv, lds_kv, st, P, S);
     } else {
       if (Tq > 0) sk_launch(&sk_dq_kernel<bf16_t, HD>, gq, lds, st, P);
-      sk_launch(&sk_dkv_kernel<bf16_t, HD>, gkv, lds_kv, st, P);
+      sk_launch(&sk_dkv_kernel<bf16_t, HD>, gkv, lds_kv, st, P, S);
     }
   });
+  sum_sinks();
   FSI_HIP_LAUNCH_CHECK("sink_attn_bwd");
   return FSI_OK;
 }

@@ -84,6 +84,20 @@ def test_longer_rows(fsi, dev, dtype, hd):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("hd,Hq,Hkv,Tq,Tk,window,sinks,lengths", [
+    (64, 2, 1, 1500, 1500, 64, 70, None),  # sinks over two tiles
+    (128, 3, 1, 1290, 1400, 100, 4, [1333]),  # fewer queries than keys, padded
+    (80, 2, 2, 1217, 1217, 0, 5, None),
+])
+def test_sinks_seen_from_afar(fsi, dev, dtype, hd, Hq, Hkv, Tq, Tk, window, sinks, lengths):
+    """Sink rows whose gradients come in several parts."""
+    q, k, v, dout = _inputs(1, Hq, Hkv, Tq, Tk, hd, dtype, seed=Tq)
+    n = None if lengths is None else torch.tensor(lengths)
+    got = _run(fsi, dev, q, k, v, dout, window=window, sinks=sinks, lengths=None if n is None else n.to(dev))
+    _check(got, *oracle.attention(q, k, v, dout, window, sinks, n, 1 / math.sqrt(hd), *UNIT[dtype]))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_memory_behind_the_lengths_is_not_used(fsi, dev, dtype):
     q, k, v, dout = _inputs(2, 2, 1, 150, 150, 64, dtype, seed=3)
     lengths = torch.tensor([100, 1])
