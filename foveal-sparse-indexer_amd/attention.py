@@ -238,8 +238,13 @@ class FovealKVCache:
             v = v.contiguous()
         _lib.require_gpu(k, v, self.k_cache, what=what)
         if self.kv_format is not None:
-            _kv_mx_write_op(k.detach(), v.detach(), _lib.KV_FORMATS[self.kv_format], rows, int(start),
-                            self.page_table, self.max_pages, self.n_phys_pages, self.k_cache, self.v_cache)
+            args = (k.detach(), v.detach(), _lib.KV_FORMATS[self.kv_format], rows, int(start), self.page_table,
+                    self.max_pages, self.n_phys_pages, self.k_cache, self.v_cache)
+            if _lib._plain_call(args):  # the launch itself, with what the dispatcher would have done beside it
+                _kv_mx_write_launch(*args)
+                torch.autograd.graph.increment_version((self.k_cache, self.v_cache))
+            else:
+                _kv_mx_write_op(*args)
             return
         _kv_write_op(k, v, int(start), self.page_table, self.max_pages, self.n_phys_pages, self.k_cache, self.v_cache)
 
@@ -330,10 +335,8 @@ def _kv_read_op(k_cache: Tensor, v_cache: Tensor, rows: Tensor, heads: int, n: i
     return k, v
 
 
-@_lib.fsi_op("kv_mx_write", lambda k, v, fmt, rows, start, page_table, max_pages, n_phys, k_cache, v_cache: None,
-             mutates_args=("k_cache", "v_cache"))
-def _kv_mx_write_op(k: Tensor, v: Tensor, fmt: int, rows: Optional[Tensor], start: int, page_table: Tensor,
-                    max_pages: int, n_phys: int, k_cache: Tensor, v_cache: Tensor) -> None:
+def _kv_mx_write_launch(k: Tensor, v: Tensor, fmt: int, rows: Optional[Tensor], start: int, page_table: Tensor,
+                        max_pages: int, n_phys: int, k_cache: Tensor, v_cache: Tensor) -> None:
     """fsi_kv_mx_write: (B, H, n, hd) K/V at positions rows[b] (or start) .. into 8- or 4-bit pages."""
     what = "FovealKVCache"
     dev = k.device
@@ -349,6 +352,10 @@ def _kv_mx_write_op(k: Tensor, v: Tensor, fmt: int, rows: Optional[Tensor], star
     if _lib.checks_enabled():
         _lib.raise_device_errors(dev, what)
 
+
+_kv_mx_write_op = _lib.fsi_op(
+    "kv_mx_write", lambda k, v, fmt, rows, start, page_table, max_pages, n_phys, k_cache, v_cache: None,
+    mutates_args=("k_cache", "v_cache"))(_kv_mx_write_launch)
 
 _CODE_DTYPES = {_lib.DTYPE_F32: torch.float32, _lib.DTYPE_BF16: torch.bfloat16}
 

@@ -24,6 +24,8 @@ struct MxParams {
   void* k_out;  // read: contiguous (B, Hkv, n_tok, HD)
   void* v_out;
   int* err;
+  unsigned pages;  // workgroups per (sequence, head)
+  bool vec;  // write: every row of K and V starts 16-byte aligned
 };
 
 template <typename T>
@@ -32,108 +34,200 @@ template <>
 __device__ __forceinline__ float mx_ld<float>(const float* p) { return *p; }
 template <>
 __device__ __forceinline__ float mx_ld<bf16_t>(const bf16_t* p) { return bf16_to_f32(*p); }
-template <typename T>
-__device__ __forceinline__ void mx_st(T* p, float x);
-template <>
-__device__ __forceinline__ void mx_st<float>(float* p, float x) { *p = x; }
-template <>
-__device__ __forceinline__ void mx_st<bf16_t>(bf16_t* p, float x) { *p = f32_to_bf16(x); }
-
-// Physical page of sequence b's token p, or -1 outside the table or the pool.
-__device__ __forceinline__ int64_t mx_phys(const MxParams& P, int b, int p) {
-  if (p < 0 || p / MX_PAGE >= P.max_pages) return -1;
-  const int64_t phys = P.page_table[static_cast<int64_t>(b) * P.max_pages + p / MX_PAGE];
-  return phys >= 0 && phys < P.n_phys ? phys : -1;
+// Largest of a lane quad (DPP, no LDS).
+__device__ __forceinline__ uint32_t quad_max(uint32_t x) {
+  const uint32_t y = __builtin_amdgcn_mov_dpp(x, 0xB1, 0xF, 0xF, true);  // lane ^ 1
+  x = x > y ? x : y;
+  const uint32_t z = __builtin_amdgcn_mov_dpp(x, 0x4E, 0xF, 0xF, true);  // lane ^ 2
+  return x > z ? x : z;
 }
 
-// One thread per (sequence, head, token, group).
-template <typename T, int FMT>
-__global__ __launch_bounds__(256) void mx_write_kernel(MxParams P) {
-  constexpr int W2 = 2 * MxFmt<FMT>::BITS / 8;
-  const int ng = P.hd / MX_GROUP;
-  const int64_t total = static_cast<int64_t>(P.B) * P.Hkv * P.n_tok * ng;
-  for (int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; id < total;
-       id += static_cast<int64_t>(gridDim.x) * 256) {
-    const int i = static_cast<int>(id % ng);
-    int64_t rest = id / ng;
-    const int t = static_cast<int>(rest % P.n_tok);
-    rest /= P.n_tok;
-    const int g = static_cast<int>(rest % P.Hkv), b = static_cast<int>(rest / P.Hkv);
-    const int64_t p = static_cast<int64_t>(P.start_rows ? P.start_rows[b] : P.start) + t;
-    const int64_t phys = p > 0x7fffffff ? -1 : mx_phys(P, b, static_cast<int>(p));
-    if (phys < 0) {
-      set_error(P.err, FSI_ERR_INDEX_RANGE);
-      continue;
+// 8 consecutive elements as fp32; vec: 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ void mx_ld8(const T* p, bool vec, float (&x)[8]) {
+  if (!vec) {
+#pragma unroll
+    for (int d = 0; d < 8; ++d) x[d] = mx_ld(p + d);
+  } else if constexpr (sizeof(T) == 4) {
+    const f32x4_t a = reinterpret_cast<const f32x4_t*>(p)[0], c = reinterpret_cast<const f32x4_t*>(p)[1];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      x[d] = a[d];
+      x[4 + d] = c[d];
     }
-    const int off = static_cast<int>(p) % MX_PAGE;
-    const int64_t base = (phys * P.Hkv + g) * mx_block_bytes(FMT, P.hd);
+  } else {
+    const u32x4_t a = *reinterpret_cast<const u32x4_t*>(p);
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-      const T* src = (kv ? static_cast<const T*>(P.v) + b * P.vs_b + g * P.vs_g + t * P.vs_t
-                         : static_cast<const T*>(P.k) + b * P.ks_b + g * P.ks_g + t * P.ks_t) + MX_GROUP * i;
-      float x[MX_GROUP];
-      uint32_t amax = 0;
-#pragma unroll
-      for (int d = 0; d < MX_GROUP; ++d) {
-        x[d] = mx_ld(src + d);
-        const uint32_t a = __float_as_uint(x[d]) & 0x7fffffffu;
-        amax = a > amax ? a : amax;
-      }
-      const int byte = mx_scale_byte<FMT>(amax);
-      const float inv = byte == SCALE_NAN ? 0.f : mx_inv_scale(byte);
-      uint8_t* blk = (kv ? P.v_pool : P.k_pool) + base;
-      uint8_t* scales = blk + mx_codes_bytes(FMT, P.hd);
-      scales[kv ? v_scale_off(ng, i, off) : k_scale_off(i, off)] = static_cast<uint8_t>(byte);
-#pragma unroll
-      for (int r = 0; r < MX_GROUP / 2; ++r) {
-        const uint32_t c0 = byte == SCALE_NAN ? 0u : mx_code<FMT>(x[2 * r] * inv);
-        const uint32_t c1 = byte == SCALE_NAN ? 0u : mx_code<FMT>(x[2 * r + 1] * inv);
-        uint8_t* dst = blk + (kv ? v_pair_off<W2>(i, r, off) : (off * P.hd + MX_GROUP * i + 2 * r) * W2 / 2);
-        if (FMT == FMT_FP4) *dst = static_cast<uint8_t>(c0 | (c1 << 4));
-        else *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(c0 | (c1 << 8));
-      }
+    for (int w = 0; w < 4; ++w) {
+      x[2 * w] = lo_bf16(a[w]);
+      x[2 * w + 1] = hi_bf16(a[w]);
     }
   }
 }
+template <typename T>
+__device__ __forceinline__ void mx_st8(T* p, const float (&x)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<f32x4_t*>(p)[0] = f32x4_t{x[0], x[1], x[2], x[3]};
+    reinterpret_cast<f32x4_t*>(p)[1] = f32x4_t{x[4], x[5], x[6], x[7]};
+  } else {
+    *reinterpret_cast<u32x4_t*>(p) = u32x4_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                                             pack_bf16x2(x[6], x[7])};
+  }
+}
 
-// One thread per (sequence, head, token, group): tokens [0, n_tok) of every sequence; 0 where the
-// page is not there.
-template <typename T, int FMT>
-__global__ __launch_bounds__(256) void mx_read_kernel(MxParams P) {
-  constexpr int W2 = 2 * MxFmt<FMT>::BITS / 8;
-  const int ng = P.hd / MX_GROUP;
-  const int64_t total = static_cast<int64_t>(P.B) * P.Hkv * P.n_tok * ng;
-  for (int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; id < total;
-       id += static_cast<int64_t>(gridDim.x) * 256) {
-    const int i = static_cast<int>(id % ng);
-    int64_t rest = id / ng;
-    const int t = static_cast<int>(rest % P.n_tok);
-    rest /= P.n_tok;
-    const int g = static_cast<int>(rest % P.Hkv), b = static_cast<int>(rest / P.Hkv);
-    const int64_t phys = mx_phys(P, b, t);
-    const int off = t % MX_PAGE;
-    const int64_t base = (phys * P.Hkv + g) * mx_block_bytes(FMT, P.hd);
-    const int64_t at = (id / ng) * P.hd + MX_GROUP * i;
+// Quantise the lane's 8 dims of a group whose other dims the lanes of its quad hold: the codes of
+// dim pair e (2 bits / 8 bytes each), the scale byte returned.
+template <int FMT>
+__device__ __forceinline__ int mx_quantise8(const float (&x)[8], uint32_t (&pair)[4]) {
+  uint32_t amax = 0;
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-      T* dst = static_cast<T*>(kv ? P.v_out : P.k_out) + at;
-      if (phys < 0) {
+  for (int d = 0; d < 8; ++d) {
+    const uint32_t a = __float_as_uint(x[d]) & 0x7fffffffu;
+    amax = a > amax ? a : amax;
+  }
+  const int byte = mx_scale_byte<FMT>(quad_max(amax));
+  const float inv = byte == SCALE_NAN ? 0.f : mx_inv_scale(byte);
 #pragma unroll
-        for (int d = 0; d < MX_GROUP; ++d) mx_st(dst + d, 0.f);
-        continue;
+  for (int e = 0; e < 4; ++e)
+    pair[e] = byte == SCALE_NAN
+                  ? 0u
+                  : mx_code<FMT>(x[2 * e] * inv) | (mx_code<FMT>(x[2 * e + 1] * inv) << MxFmt<FMT>::BITS);
+  return byte;
+}
+
+constexpr int MX_THREADS = 256;
+
+// A workgroup writes its share of one (page, head): a thread takes 8 dims of a token, a lane quad
+// a group.  K's codes go straight to memory (a token's row is contiguous); V's codes and both
+// scales are laid out in LDS, and leave as 16-byte pieces of a page that is written whole, as
+// single pairs and bytes otherwise.
+template <typename T, int FMT, int HD>
+__global__ __launch_bounds__(MX_THREADS) void mx_write_kernel(MxParams P) {
+  constexpr int BITS = MxFmt<FMT>::BITS, W2 = 2 * BITS / 8, NG = HD / MX_GROUP, TPT = HD / 8;
+  constexpr int CODES = MX_PAGE * HD * BITS / 8, SCALES = MX_PAGE * NG;
+  __shared__ __attribute__((aligned(16))) uint8_t vimg[CODES + SCALES];
+  __shared__ __attribute__((aligned(16))) uint8_t kscale[SCALES];
+  const int bh = static_cast<int>(blockIdx.x / P.pages), g = bh % P.Hkv, b = bh / P.Hkv;
+  const int64_t start = P.start_rows ? P.start_rows[b] : P.start;
+  // the page that holds position start (rounded down for negative ones), then the later ones
+  const int64_t page = (start >= 0 ? start / MX_PAGE : -((MX_PAGE - 1 - start) / MX_PAGE)) + blockIdx.x % P.pages;
+  const int64_t t_base = page * MX_PAGE - start;  // input token of the page's first slot
+  const int lo = t_base < 0 ? static_cast<int>(-t_base) : 0;
+  const int hi = P.n_tok - t_base < MX_PAGE ? static_cast<int>(P.n_tok - t_base) : MX_PAGE;
+  if (hi <= lo) return;
+  int64_t phys = -1;
+  if (page >= 0 && page < P.max_pages) phys = P.page_table[static_cast<int64_t>(b) * P.max_pages + page];
+  if (phys < 0 || phys >= P.n_phys) {
+    if (threadIdx.x == 0) set_error(P.err, FSI_ERR_INDEX_RANGE);
+    return;
+  }
+  const int64_t base = (phys * P.Hkv + g) * (CODES + SCALES);
+  const T* k = static_cast<const T*>(P.k) + b * P.ks_b + g * P.ks_g;
+  const T* v = static_cast<const T*>(P.v) + b * P.vs_b + g * P.vs_g;
+  const int piece = threadIdx.x % TPT, d0 = 8 * piece, group = piece / 4;
+  // hd 96: 21 tokens of 12 threads a round; the last 4 threads idle
+  for (int t = lo + static_cast<int>(threadIdx.x) / TPT; t < hi; t += MX_THREADS / TPT) {
+    if (threadIdx.x >= MX_THREADS / TPT * TPT) break;
+    const int64_t src = t_base + t;
+    float x[8], y[8];
+    mx_ld8(k + src * P.ks_t + d0, P.vec, x);
+    mx_ld8(v + src * P.vs_t + d0, P.vec, y);
+    uint32_t pair[4];
+    const int kb = mx_quantise8<FMT>(x, pair);
+    uint8_t* kd = P.k_pool + base + (t * HD + d0) * BITS / 8;
+    if constexpr (FMT == FMT_FP4) {
+      *reinterpret_cast<uint32_t*>(kd) = pair[0] | (pair[1] << 8) | (pair[2] << 16) | (pair[3] << 24);
+    } else {
+      *reinterpret_cast<u32x2_t*>(kd) = u32x2_t{pair[0] | (pair[1] << 16), pair[2] | (pair[3] << 16)};
+    }
+    const int vb = mx_quantise8<FMT>(y, pair);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      uint8_t* vd = vimg + v_pair_off<W2>(group, (piece % 4) * 4 + e, t);
+      if constexpr (FMT == FMT_FP4) *vd = static_cast<uint8_t>(pair[e]);
+      else *reinterpret_cast<uint16_t*>(vd) = static_cast<uint16_t>(pair[e]);
+    }
+    if (piece % 4 == 0) {
+      kscale[k_scale_off(group, t)] = static_cast<uint8_t>(kb);
+      vimg[CODES + v_scale_off(NG, group, t)] = static_cast<uint8_t>(vb);
+    }
+  }
+  __syncthreads();
+  uint8_t* kdst = P.k_pool + base + CODES;
+  uint8_t* vdst = P.v_pool + base;
+  if (lo == 0 && hi == MX_PAGE) {
+    for (int i = threadIdx.x; i < (CODES + SCALES) / 16; i += MX_THREADS)
+      reinterpret_cast<u32x4_t*>(vdst)[i] = reinterpret_cast<const u32x4_t*>(vimg)[i];
+    for (int i = threadIdx.x; i < SCALES / 16; i += MX_THREADS)
+      reinterpret_cast<u32x4_t*>(kdst)[i] = reinterpret_cast<const u32x4_t*>(kscale)[i];
+    return;
+  }
+  for (int i = threadIdx.x; i < (hi - lo) * (HD / 2); i += MX_THREADS) {
+    const int t = lo + i / (HD / 2), pr = i % (HD / 2), at = v_pair_off<W2>(pr / 16, pr % 16, t);
+    if constexpr (FMT == FMT_FP4) vdst[at] = vimg[at];
+    else *reinterpret_cast<uint16_t*>(vdst + at) = *reinterpret_cast<const uint16_t*>(vimg + at);
+  }
+  for (int i = threadIdx.x; i < (hi - lo) * NG; i += MX_THREADS) {
+    const int t = lo + i / NG, gi = i % NG;
+    kdst[k_scale_off(gi, t)] = kscale[k_scale_off(gi, t)];
+    vdst[CODES + v_scale_off(NG, gi, t)] = vimg[CODES + v_scale_off(NG, gi, t)];
+  }
+}
+
+// One page of a head back to rows: V's block through LDS, 8 dims of a token a thread.  0 where
+// the page is not there.
+template <typename T, int FMT, int HD>
+__global__ __launch_bounds__(MX_THREADS) void mx_read_kernel(MxParams P) {
+  constexpr int BITS = MxFmt<FMT>::BITS, W2 = 2 * BITS / 8, NG = HD / MX_GROUP, TPT = HD / 8;
+  constexpr int CODES = MX_PAGE * HD * BITS / 8, SCALES = MX_PAGE * NG;
+  __shared__ __attribute__((aligned(16))) uint8_t vimg[CODES + SCALES];
+  const int bh = static_cast<int>(blockIdx.x / P.pages), g = bh % P.Hkv, b = bh / P.Hkv;
+  const int page = static_cast<int>(blockIdx.x % P.pages);
+  const int hi = P.n_tok - page * MX_PAGE < MX_PAGE ? P.n_tok - page * MX_PAGE : MX_PAGE;
+  int64_t phys = page < P.max_pages ? P.page_table[static_cast<int64_t>(b) * P.max_pages + page] : -1;
+  if (phys >= P.n_phys) phys = -1;
+  const int64_t base = (phys * P.Hkv + g) * (CODES + SCALES);
+  if (phys >= 0) {
+    for (int i = threadIdx.x; i < (CODES + SCALES) / 16; i += MX_THREADS)
+      reinterpret_cast<u32x4_t*>(vimg)[i] = reinterpret_cast<const u32x4_t*>(P.v_pool + base)[i];
+  }
+  __syncthreads();
+  const int piece = threadIdx.x % TPT, d0 = 8 * piece, group = piece / 4;
+  const int64_t row0 = (static_cast<int64_t>(b) * P.Hkv + g) * P.n_tok + static_cast<int64_t>(page) * MX_PAGE;
+  const float nan = __uint_as_float(0x7fc00000u);
+  for (int t = static_cast<int>(threadIdx.x) / TPT; t < hi; t += MX_THREADS / TPT) {
+    if (threadIdx.x >= MX_THREADS / TPT * TPT) break;
+    float x[8], y[8];
+    if (phys < 0) {
+#pragma unroll
+      for (int d = 0; d < 8; ++d) x[d] = y[d] = 0.f;
+    } else {
+      const uint8_t* kb = P.k_pool + base;
+      const int ks = kb[CODES + k_scale_off(group, t)], vs = vimg[CODES + v_scale_off(NG, group, t)];
+      const float fk = ks == SCALE_NAN ? nan : mx_scale(ks), fv = vs == SCALE_NAN ? nan : mx_scale(vs);
+      uint32_t w[2];
+      const uint8_t* ksrc = kb + (t * HD + d0) * BITS / 8;
+      if constexpr (FMT == FMT_FP4) {
+        w[0] = w[1] = *reinterpret_cast<const uint32_t*>(ksrc);
+      } else {
+        const u32x2_t z = *reinterpret_cast<const u32x2_t*>(ksrc);
+        w[0] = z[0];
+        w[1] = z[1];
       }
-      const uint8_t* blk = (kv ? P.v_pool : P.k_pool) + base;
-      const int byte = blk[mx_codes_bytes(FMT, P.hd) + (kv ? v_scale_off(ng, i, off) : k_scale_off(i, off))];
-      const float s = byte == SCALE_NAN ? __uint_as_float(0x7fc00000u) : mx_scale(byte);
 #pragma unroll
-      for (int r = 0; r < MX_GROUP / 2; ++r) {
-        const uint8_t* src = blk + (kv ? v_pair_off<W2>(i, r, off) : (off * P.hd + MX_GROUP * i + 2 * r) * W2 / 2);
-        const uint32_t c = FMT == FMT_FP4 ? *src : *reinterpret_cast<const uint16_t*>(src);
-        const uint32_t c0 = FMT == FMT_FP4 ? c & 15u : c & 255u, c1 = FMT == FMT_FP4 ? c >> 4 : c >> 8;
-        mx_st(dst + 2 * r, mx_value<FMT>(c0) * s);
-        mx_st(dst + 2 * r + 1, mx_value<FMT>(c1) * s);
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t ck = FMT == FMT_FP4 ? w[0] >> (8 * e) : w[e >> 1] >> (16 * (e & 1));
+        const uint8_t* vsrc = vimg + v_pair_off<W2>(group, (piece % 4) * 4 + e, t);
+        const uint32_t cv = FMT == FMT_FP4 ? *vsrc : *reinterpret_cast<const uint16_t*>(vsrc);
+        x[2 * e] = mx_value<FMT>(ck & ((1u << BITS) - 1)) * fk;
+        x[2 * e + 1] = mx_value<FMT>((ck >> BITS) & ((1u << BITS) - 1)) * fk;
+        y[2 * e] = mx_value<FMT>(cv & ((1u << BITS) - 1)) * fv;
+        y[2 * e + 1] = mx_value<FMT>((cv >> BITS) & ((1u << BITS) - 1)) * fv;
       }
     }
+    const int64_t at = (row0 + t) * HD + d0;
+    mx_st8(static_cast<T*>(P.k_out) + at, x);
+    mx_st8(static_cast<T*>(P.v_out) + at, y);
   }
 }
 
@@ -145,21 +239,28 @@ int mx_check(const char* what, int64_t B, int64_t Hkv, int64_t n_tok, int64_t he
                 what, (long long)head_dim);
   FSI_CHECK_ARG(B >= 0 && Hkv > 0 && n_tok >= 0 && max_pages > 0 && n_phys_pages > 0, FSI_ERR_SHAPE, "%s: bad sizes",
                 what);
-  FSI_CHECK_ARG(max_pages <= 0x7fffffff / MX_PAGE && B <= 0x7fffffff && Hkv <= 0x7fffffff && n_tok <= 0x7fffffff,
+  FSI_CHECK_ARG(max_pages <= 0x7fffffff / MX_PAGE && B <= 0x7fffffff && Hkv <= 0x7fffffff && n_tok <= 0x7fffff00,
                 FSI_ERR_SHAPE, "%s: sizes beyond int32", what);
   return FSI_OK;
 }
 
-// f(type tag, format tag) for the call's type and format.
+// f(type tag, format tag, head size tag) for the call's type, format and head size.
 template <typename F>
-void mx_dispatch(int dtype, int format, F&& f) {
-  if (dtype == FSI_DTYPE_F32) {
-    if (format == FSI_KV_MXFP4) f(float{}, std::integral_constant<int, FMT_FP4>{});
-    else f(float{}, std::integral_constant<int, FMT_FP8>{});
-  } else {
-    if (format == FSI_KV_MXFP4) f(bf16_t{}, std::integral_constant<int, FMT_FP4>{});
-    else f(bf16_t{}, std::integral_constant<int, FMT_FP8>{});
-  }
+void mx_dispatch(int dtype, int format, int64_t hd, F&& f) {
+  auto by_hd = [&](auto t, auto fm) {
+    switch (hd) {
+      case 64: f(t, fm, std::integral_constant<int, 64>{}); break;
+      case 96: f(t, fm, std::integral_constant<int, 96>{}); break;
+      case 128: f(t, fm, std::integral_constant<int, 128>{}); break;
+      default: f(t, fm, std::integral_constant<int, 256>{});
+    }
+  };
+  auto by_format = [&](auto t) {
+    if (format == FSI_KV_MXFP4) by_hd(t, std::integral_constant<int, FMT_FP4>{});
+    else by_hd(t, std::integral_constant<int, FMT_FP8>{});
+  };
+  if (dtype == FSI_DTYPE_F32) by_format(float{});
+  else by_format(bf16_t{});
 }
 
 }  // namespace
@@ -205,10 +306,16 @@ FSI_API int fsi_kv_mx_write(const void* k, const void* v, int64_t k_stride_b, in
   P.k_pool = static_cast<uint8_t*>(k_pool);
   P.v_pool = static_cast<uint8_t*>(v_pool);
   P.err = err;
-  const int64_t total = B * Hkv * n_tok * (head_dim / MX_GROUP);
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>((total + 255) / 256, 1 << 20));
-  mx_dispatch(dtype, format, [&](auto t, auto f) {
-    mx_write_kernel<decltype(t), decltype(f)::value><<<grid, 256, 0, reinterpret_cast<hipStream_t>(stream)>>>(P);
+  const int64_t esz = dtype == FSI_DTYPE_F32 ? 4 : 2;
+  P.vec = (reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 == 0 &&
+          ((k_stride_b | k_stride_h | k_stride_t | v_stride_b | v_stride_h | v_stride_t) * esz) % 16 == 0;
+  // the pages that n_tok tokens touch at most, from any start
+  P.pages = static_cast<unsigned>((n_tok + MX_PAGE - 2) / MX_PAGE + 1);
+  FSI_CHECK_ARG(B * Hkv <= 0x7fffffff / P.pages, FSI_ERR_SHAPE, "kv_mx_write: B * Hkv * tokens beyond the grid");
+  const unsigned grid = static_cast<unsigned>(B * Hkv) * P.pages;
+  mx_dispatch(dtype, format, head_dim, [&](auto t, auto f, auto hd) {
+    mx_write_kernel<decltype(t), decltype(f)::value, decltype(hd)::value>
+        <<<grid, MX_THREADS, 0, reinterpret_cast<hipStream_t>(stream)>>>(P);
   });
   FSI_HIP_LAUNCH_CHECK("kv_mx_write");
   return FSI_OK;
@@ -236,10 +343,12 @@ FSI_API int fsi_kv_mx_read(const void* k_pool, const void* v_pool, int format, i
   P.v_pool = static_cast<uint8_t*>(const_cast<void*>(v_pool));
   P.k_out = k_out;
   P.v_out = v_out;
-  const int64_t total = B * Hkv * n_tok * (head_dim / MX_GROUP);
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>((total + 255) / 256, 1 << 20));
-  mx_dispatch(dtype, format, [&](auto t, auto f) {
-    mx_read_kernel<decltype(t), decltype(f)::value><<<grid, 256, 0, reinterpret_cast<hipStream_t>(stream)>>>(P);
+  P.pages = static_cast<unsigned>((n_tok + MX_PAGE - 1) / MX_PAGE);
+  FSI_CHECK_ARG(B * Hkv <= 0x7fffffff / P.pages, FSI_ERR_SHAPE, "kv_mx_read: B * Hkv * tokens beyond the grid");
+  const unsigned grid = static_cast<unsigned>(B * Hkv) * P.pages;
+  mx_dispatch(dtype, format, head_dim, [&](auto t, auto f, auto hd) {
+    mx_read_kernel<decltype(t), decltype(f)::value, decltype(hd)::value>
+        <<<grid, MX_THREADS, 0, reinterpret_cast<hipStream_t>(stream)>>>(P);
   });
   FSI_HIP_LAUNCH_CHECK("kv_mx_read");
   return FSI_OK;
