@@ -499,20 +499,29 @@ __global__ void md_merge_kernel(MdParams P, int hd) {
   else static_cast<float*>(P.out)[at] = x;
 }
 
-// Waves per (sequence, KV head, 16 query heads) and the workgroups that hold them.
+// Waves per workgroup and workgroups per (sequence, KV head, 16 query heads), a pair below.
+// Eight waves a CU stream with enough loads in flight, so one round of workgroups holds
+// MD_SLOTS = 256 CUs x 8 waves.  Where the pairs alone give that, a pair is one workgroup of up
+// to 8 waves and needs no merge; fewer pairs are cut into workgroups of 4 waves, as many as one
+// round holds (a second round of a few workgroups would double the time), and no more than the
+// chunks per wave that results needs.
 struct MdSplit {
   int waves, wgs;
 };
-constexpr int64_t MD_TARGET_WAVES = 2048;
+constexpr int64_t MD_SLOTS = 2048;
 MdSplit md_split(int64_t pairs, int64_t hd, int format, int64_t window, int64_t sinks, int64_t cap,
                  int64_t max_pages) {
   const int64_t tok = md_tok(format, hd);
   const int64_t all = max_pages * (MX_PAGE / tok);
   const int64_t local = std::min<int64_t>(window / tok + 2, all);
   const int64_t chunks = std::min<int64_t>((sinks + tok - 1) / tok, all) + local + cap * (MX_PAGE / tok);
-  int64_t s = std::min<int64_t>(std::max<int64_t>((MD_TARGET_WAVES + pairs - 1) / pairs, 1), chunks);
-  if (s <= MD_MAX_WAVES) return {static_cast<int>(s), 1};
-  return {MD_MAX_WAVES, static_cast<int>((s + MD_MAX_WAVES - 1) / MD_MAX_WAVES)};
+  const int64_t most = std::max<int64_t>(MD_SLOTS / pairs, 1);  // waves a pair may have
+  if (chunks <= MD_MAX_WAVES || most <= MD_MAX_WAVES)
+    return {static_cast<int>(std::min<int64_t>({chunks, most, MD_MAX_WAVES})), 1};
+  const int64_t wgs = std::min<int64_t>(most / 4, (chunks + 3) / 4);
+  const int64_t per = (chunks + 4 * wgs - 1) / (4 * wgs);
+  const int64_t need = (chunks + 4 * per - 1) / (4 * per);
+  return need <= 2 ? MdSplit{MD_MAX_WAVES, 1} : MdSplit{4, static_cast<int>(need)};
 }
 
 int64_t md_subs(int64_t Hq, int64_t Hkv) { return (Hq / Hkv + 15) / 16; }
