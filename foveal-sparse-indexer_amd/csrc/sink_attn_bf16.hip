@@ -22,11 +22,15 @@ namespace {
 static_assert(SK_T == AB_T, "one tile size");
 constexpr float SB_LOG2E = 1.4426950408889634f;
 
-// dims 32 s + 8 kg .. of row `row` of a (., HD) matrix
+// dims 32 s + 8 kg .. of row `row` of a (., HD) matrix; 0 where !ok (row is then any row that exists)
 template <int HD>
-__device__ __forceinline__ void sb_frag(const bf16_t* base, int64_t rs, int row, int kg, u32x4_t (&f)[HD / 32]) {
+__device__ __forceinline__ void sb_frag(const bf16_t* base, int64_t rs, int row, bool ok, int kg,
+                                        u32x4_t (&f)[HD / 32]) {
 #pragma unroll
-  for (int s = 0; s < HD / 32; ++s) f[s] = *reinterpret_cast<const u32x4_t*>(base + row * rs + 32 * s + 8 * kg);
+  for (int s = 0; s < HD / 32; ++s) {
+    const u32x4_t x = *reinterpret_cast<const u32x4_t*>(base + row * rs + 32 * s + 8 * kg);
+    f[s] = ok ? x : u32x4_t{0u, 0u, 0u, 0u};
+  }
 }
 
 // How the keys [a, a + n) of a tile meet the queries at positions [p0, p1] (both uniform).
@@ -38,21 +42,23 @@ __device__ __forceinline__ SbKeys sb_keys(const SkParams& P, int len, int a, int
 }
 
 // ---------------------------------------------------------------------------
-// Forward.  A workgroup of 8 waves is HPW query heads of one KV head (they share the K / V
-// tiles) at 32 * 8 / HPW queries; a wave is one head's 32 queries (two 16-query tiles, so a K or
-// V fragment read from LDS enters two MFMAs).  Two key tiles are computed per barrier while the
-// next two load.
+// Forward.  A workgroup of 4 waves is HPW query heads of one KV head (they share the K / V
+// tiles) at 32 * 4 / HPW queries; a wave is one head's 32 queries (two 16-query tiles, so a K or
+// V fragment read from LDS enters two MFMAs).  Two workgroups a CU: the two waves of a SIMD then
+// meet no common barrier, and one's products run beside the other's softmax (8 waves a workgroup
+// over a ring of four tiles: 2 x 4096 tokens 190 against 168 us, 16384 tokens 2 % slower).
 // The running maximum moves only when a score exceeds it by more than 2^8: P then stays below
 // 2^8, most tiles need one compare instead of the row maxima, and the accumulators are rescaled
 // rarely.
 // ---------------------------------------------------------------------------
-constexpr int SB_FWD_THREADS = 512;
+constexpr int SB_THREADS = 256;
+constexpr int SB_WAVES = SB_THREADS / 64;
 
 template <int HD, int HPW, bool LSE>
-__global__ __launch_bounds__(SB_FWD_THREADS, 2) void sb_fwd_kernel(SkParams P) {
+__global__ __launch_bounds__(SB_THREADS, 2) void sb_fwd_kernel(SkParams P) {
   constexpr int KS = HD / 32, DT = HD / 16, TB = sab_tile_bytes<HD>();
-  constexpr int QW = 8 / HPW * 32;  // queries of a workgroup
-  __shared__ __attribute__((aligned(1024))) char smem[4 * 2 * TB];  // [stage][K, V]
+  constexpr int QW = SB_WAVES / HPW * 32;  // queries of a workgroup
+  __shared__ __attribute__((aligned(1024))) char smem[2 * 2 * TB];  // [stage][K, V]
   const int per = P.Hq / HPW;  // workgroups a query range takes
   const int hp = static_cast<int>(blockIdx.x) % per, b = blockIdx.y;
   const int i0 = (static_cast<int>(gridDim.x) / per - 1 - static_cast<int>(blockIdx.x) / per) * QW;
@@ -69,19 +75,20 @@ __global__ __launch_bounds__(SB_FWD_THREADS, 2) void sb_fwd_kernel(SkParams P) {
   const int n = tiles.count();
   auto load = [&](int c) {
     if (c >= n) return;
-    char* dst = smem + (c & 3) * (2 * TB);
-    sab_dma<HD, SB_FWD_THREADS>(k, P.ks_t, tiles.tile(c) * SK_T, len, dst);
-    sab_dma<HD, SB_FWD_THREADS>(v, P.vs_t, tiles.tile(c) * SK_T, len, dst + TB);
+    char* dst = smem + (c & 1) * (2 * TB);
+    sab_dma<HD, SB_THREADS>(k, P.ks_t, tiles.tile(c) * SK_T, len, dst);
+    sab_dma<HD, SB_THREADS>(v, P.vs_t, tiles.tile(c) * SK_T, len, dst + TB);
   };
   load(0);
-  load(1);
   u32x4_t q[2][KS];
   int hi[2];  // last visible key of query iw + 16 i + r
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int qi = iw + 16 * i + r;
-    sb_frag<HD>(static_cast<const bf16_t*>(P.q) + b * P.qs_b + h * P.qs_h, P.qs_t, qi < P.Tq ? qi : P.Tq - 1, kg, q[i]);
-    hi[i] = qi < P.Tq && off + qi < len ? off + qi : -1;
+    const bool live = qi < P.Tq && off + qi < len;
+    sb_frag<HD>(static_cast<const bf16_t*>(P.q) + b * P.qs_b + h * P.qs_h, P.qs_t, qi < P.Tq ? qi : P.Tq - 1, live, kg,
+                q[i]);
+    hi[i] = live ? off + qi : -1;
   }
   const float sl2 = P.scale * SB_LOG2E, inv_sl2 = 1.f / sl2;
   f32x4_t acc[2][DT], lsum[2];
@@ -99,7 +106,7 @@ __global__ __launch_bounds__(SB_FWD_THREADS, 2) void sb_fwd_kernel(SkParams P) {
 
   auto step = [&](int c) {
     const int s0 = tiles.tile(c) * SK_T;
-    const uint32_t at = (c & 3) * (2 * TB);
+    const uint32_t at = (c & 1) * (2 * TB);
     const SbKeys all = sb_keys(P, len, s0, SK_T, pw, pw1);
     if (all == SB_NONE) return;
     f32x4_t st[2][4];
@@ -177,12 +184,10 @@ __global__ __launch_bounds__(SB_FWD_THREADS, 2) void sb_fwd_kernel(SkParams P) {
     }
   };
 
-  __syncthreads();  // the first tiles are there
-  for (int c = 0; c < n; c += 2) {
-    load(c + 2);
-    load(c + 3);
+  __syncthreads();  // the first tile is there
+  for (int c = 0; c < n; ++c) {
+    load(c + 1);
     step(c);
-    if (c + 1 < n) step(c + 1);
     __syncthreads();
   }
 
@@ -209,12 +214,10 @@ __global__ __launch_bounds__(SB_FWD_THREADS, 2) void sb_fwd_kernel(SkParams P) {
 // dQ, and D for the key kernel.  A workgroup of 4 waves is HPW query heads of one KV head at
 // 64 * 2 / HPW queries; a wave is one head's 32 queries over 32 keys at a time.
 // ---------------------------------------------------------------------------
-constexpr int SB_THREADS = 256;
-
 template <int HD, int HPW>
 __global__ __launch_bounds__(SB_THREADS, 2) void sb_dq_kernel(SkParams P) {
   constexpr int KS = HD / 32, DT = HD / 16, TB = sab_tile_bytes<HD>();
-  constexpr int QW = 4 / HPW * 32;
+  constexpr int QW = SB_WAVES / HPW * 32;
   __shared__ __attribute__((aligned(1024))) char smem[2 * 2 * TB];  // [stage][K, V]
   const int per = P.Hq / HPW;
   const int hp = static_cast<int>(blockIdx.x) % per, b = blockIdx.y;
@@ -243,10 +246,11 @@ __global__ __launch_bounds__(SB_THREADS, 2) void sb_dq_kernel(SkParams P) {
   for (int i = 0; i < 2; ++i) {
     const int qi = iw + 16 * i + r, ql = qi < P.Tq ? qi : P.Tq - 1;
     const bool live = qi < P.Tq && off + qi < len;
-    sb_frag<HD>(static_cast<const bf16_t*>(P.q) + b * P.qs_b + h * P.qs_h, P.qs_t, ql, kg, q[i]);
-    sb_frag<HD>(static_cast<const bf16_t*>(P.dout) + b * P.ds_b + h * P.ds_h, P.ds_t, ql, kg, gr[i]);
+    sb_frag<HD>(static_cast<const bf16_t*>(P.q) + b * P.qs_b + h * P.qs_h, P.qs_t, ql, live, kg, q[i]);
+    sb_frag<HD>(static_cast<const bf16_t*>(P.dout) + b * P.ds_b + h * P.ds_h, P.ds_t, ql, live, kg,
+                gr[i]);
     u32x4_t of[KS];
-    sb_frag<HD>(static_cast<const bf16_t*>(P.o) + b * P.os_b + h * P.os_h, P.os_t, ql, kg, of);
+    sb_frag<HD>(static_cast<const bf16_t*>(P.o) + b * P.os_b + h * P.os_h, P.os_t, ql, live, kg, of);
     float d = 0.f;
 #pragma unroll
     for (int s = 0; s < KS; ++s)
@@ -255,7 +259,7 @@ __global__ __launch_bounds__(SB_THREADS, 2) void sb_dq_kernel(SkParams P) {
         d = fmaf(lo_bf16(gr[i][s][w]), lo_bf16(of[s][w]), d);
         d = fmaf(hi_bf16(gr[i][s][w]), hi_bf16(of[s][w]), d);
       }
-    dd[i] = live ? sum_rows4(d) : 0.f;
+    dd[i] = sum_rows4(d);
     lse[i] = live ? P.lse[stat + qi] : INFINITY;
     hi[i] = live ? off + qi : -1;
     if (qi < P.Tq && kg == 0) P.dd[stat + qi] = dd[i];
@@ -292,25 +296,32 @@ __global__ __launch_bounds__(SB_THREADS, 2) void sb_dq_kernel(SkParams P) {
           }
         }
       }
-      u32x4_t ds[2];
+      // the mask is a loop of its own, so that whole tiles run without branches
+      if (all != SB_ALL) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 2; ++i) {
+          const int lo = hi[i] - P.window;
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int s = a0 + 16 * t + 4 * kg + j;
+              st[i][t][j] = s <= hi[i] && (s > lo || s < P.sinks) ? st[i][t][j] : -INFINITY;
+            }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float p = __builtin_amdgcn_exp2f(fmaf(st[i][t][j], sl2, -lse[i]));
-            if (all != SB_ALL) {
-              const int s = a0 + 16 * t + 4 * kg + j;
-              p = s <= hi[i] && (s > hi[i] - P.window || s < P.sinks) ? p : 0.f;
-              st[i][t][j] = p == 0.f ? 0.f : p * (dp[i][t][j] - dd[i]);  // hidden memory may hold anything
-            } else {
-              st[i][t][j] = p * (dp[i][t][j] - dd[i]);
-            }
-          }
+          for (int j = 0; j < 4; ++j)  // dS^T
+            dp[i][t][j] = __builtin_amdgcn_exp2f(fmaf(st[i][t][j], sl2, -lse[i])) * (dp[i][t][j] - dd[i]);
+      u32x4_t ds[2];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) ds[i][w] = bf_cvt2(st[i][w >> 1][2 * (w & 1)], st[i][w >> 1][2 * (w & 1) + 1]);
-      }
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) ds[i][w] = bf_cvt2(dp[i][w >> 1][2 * (w & 1)], dp[i][w >> 1][2 * (w & 1) + 1]);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const u32x4_t a = sab_trow<HD>(smem, tr_off + at, dt, 0);
@@ -365,8 +376,8 @@ __global__ __launch_bounds__(SB_THREADS, 2) void sb_dkv_kernel(SkParams P, SkSin
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt) {
     const int s = sw + 16 * kt + r, sl = s < P.Tk ? s : P.Tk - 1;
-    sb_frag<HD>(k, P.ks_t, sl, kg, kb[kt]);
-    sb_frag<HD>(v, P.vs_t, sl, kg, vb[kt]);
+    sb_frag<HD>(k, P.ks_t, sl, s < len, kg, kb[kt]);
+    sb_frag<HD>(v, P.vs_t, sl, s < len, kg, vb[kt]);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) dka[kt][dt] = dva[kt][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
@@ -397,7 +408,6 @@ __global__ __launch_bounds__(SB_THREADS, 2) void sb_dkv_kernel(SkParams P, SkSin
     const int p0 = off + t0 + 32 * wq, p1 = off + min(t0 + 32 * wq + 32, q_end) - 1;
     const SbKeys all = sb_keys(P, len, sw, 32, p0, p1);
     if (all != SB_NONE) {
-      const bool full = all == SB_ALL && t0 + 32 * wq + 32 <= q_end;
       f32x4_t s[2][2], dp[2][2];  // [key half][16-query part]: query 32 wq + 16 i + 4 kg + e, key r
 #pragma unroll
       for (int qt = 0; qt < 2; ++qt) {
@@ -413,7 +423,21 @@ __global__ __launch_bounds__(SB_THREADS, 2) void sb_dkv_kernel(SkParams P, SkSin
           }
         }
       }
-      __builtin_amdgcn_sched_barrier(0);  // register budget: keep the phases apart
+      // the mask is a loop of its own, so that whole tiles run without branches
+      if (all != SB_ALL || t0 + 32 * wq + 32 > q_end) {
+#pragma unroll
+        for (int qt = 0; qt < 2; ++qt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int t = t0 + 32 * wq + 16 * qt + 4 * kg + e;
+            const int last = t < q_end ? off + t : -1, lo = last - P.window;
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+              const int key = sw + 16 * kt + r;
+              s[kt][qt][e] = key <= last && (key > lo || key < P.sinks) ? s[kt][qt][e] : -INFINITY;
+            }
+          }
+      }
 #pragma unroll
       for (int qt = 0; qt < 2; ++qt) {
         const int rq = 32 * wq + 16 * qt + 4 * kg;
@@ -421,24 +445,14 @@ __global__ __launch_bounds__(SB_THREADS, 2) void sb_dkv_kernel(SkParams P, SkSin
         const f32x4_t lse = *reinterpret_cast<const f32x4_t*>(rows);
         const f32x4_t rd = *reinterpret_cast<const f32x4_t*>(rows + AB_T);
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-          const int key = sw + 16 * kt + r;
+        for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float p = __builtin_amdgcn_exp2f(fmaf(s[kt][qt][e], sl2, -lse[e]));
-            if (!full) {
-              const int t = t0 + rq + e;
-              const bool ok = t < q_end && sk_visible(P, len, off + t, key);
-              p = ok ? p : 0.f;
-              dp[kt][qt][e] = ok ? p * (dp[kt][qt][e] - rd[e]) : 0.f;
-            } else {
-              dp[kt][qt][e] = p * (dp[kt][qt][e] - rd[e]);
-            }
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[kt][qt][e], sl2, -lse[e]));
+            dp[kt][qt][e] = p * (dp[kt][qt][e] - rd[e]);  // dS
             s[kt][qt][e] = p;
           }
-        }
       }
-      __builtin_amdgcn_sched_barrier(0);  // register budget: keep the phases apart
       u32x4_t ph[2], dh[2];
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
@@ -524,10 +538,10 @@ void sb_forward(const SkParams& P, hipStream_t st) {
   auto run = [&](auto hd) {
     constexpr int HD = decltype(hd)::value;
     auto launch = [&](auto heads) {
-      constexpr int HPW = decltype(heads)::value, QW = 8 / HPW * 32;
+      constexpr int HPW = decltype(heads)::value, QW = SB_WAVES / HPW * 32;
       const dim3 grid(static_cast<unsigned>((P.Tq + QW - 1) / QW * (P.Hq / HPW)), static_cast<unsigned>(P.B));
-      if (P.lse) sb_fwd_kernel<HD, HPW, true><<<grid, SB_FWD_THREADS, 0, st>>>(P);
-      else sb_fwd_kernel<HD, HPW, false><<<grid, SB_FWD_THREADS, 0, st>>>(P);
+      if (P.lse) sb_fwd_kernel<HD, HPW, true><<<grid, SB_THREADS, 0, st>>>(P);
+      else sb_fwd_kernel<HD, HPW, false><<<grid, SB_THREADS, 0, st>>>(P);
     };
     switch (sb_heads(P, 4)) {
       case 4: launch(std::integral_constant<int, 4>{}); break;
@@ -543,7 +557,7 @@ void sb_backward(const SkParams& P, const SkSinkSplit& S, hipStream_t st) {
   auto run = [&](auto hd) {
     constexpr int HD = decltype(hd)::value;
     auto launch = [&](auto heads) {
-      constexpr int HPW = decltype(heads)::value, QW = 4 / HPW * 32;
+      constexpr int HPW = decltype(heads)::value, QW = SB_WAVES / HPW * 32;
       const dim3 grid(static_cast<unsigned>((P.Tq + QW - 1) / QW * (P.Hq / HPW)), static_cast<unsigned>(P.B));
       sb_dq_kernel<HD, HPW><<<grid, SB_THREADS, 0, st>>>(P);
     };

@@ -118,8 +118,9 @@ def sink_window_attention(
     memory may hold anything.  A query that sees no key (window 0 without sinks) gets 0.
     bf16 or fp32, hd up to 256, softmax and sums in fp32; views with unit stride over hd are
     read in place.  scale defaults to 1 / sqrt(hd).  Differentiable (once) in q, k and v.
-    Hidden values of v inside a length enter as 0 times the value, so they have to be
-    finite; hidden keys may hold anything.  Returns (B, Hq, Tq, hd), a view of a
+    Inside a length, v where it is hidden enters as 0 times the value, in the gradients q, k
+    and the incoming gradient as well, so they have to be finite; hidden k may hold anything
+    in the forward.  Returns (B, Hq, Tq, hd), a view of a
     (B, Tq, Hq, hd) buffer."""
     dev = _lib.require_gpu(q, k, v, lengths, what=_WHAT)
     if not (q.dtype == k.dtype == v.dtype):
