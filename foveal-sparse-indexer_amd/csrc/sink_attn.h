@@ -33,6 +33,7 @@ struct SkParams {
   void* dq;    // contiguous gradients of the operands' type
   void* dk;
   void* dv;
+  bool vec;    // sink_attn.hip's kernels: 4 elements at a time can be read from the tiles' rows
 };
 
 __device__ __forceinline__ int sk_length(const SkParams& P, int b) {

@@ -28,15 +28,40 @@ __device__ __forceinline__ f32x4_t mfma4(float a, float b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-// Rows [r0, r0 + 64) of a (n, hd) matrix into an LDS tile of row stride HD + 4 (the pad puts the
-// 16 rows of a column read on distinct banks); rows from n on and dims from hd on read as 0.
+// Rows [r0, r0 + 64) of a (n, hd) matrix on their way into an LDS tile of row stride HD + 4 (the
+// pad puts the 16 rows of a column read on distinct banks): fetched into registers while the tile
+// before is computed, stored after it.  Rows from n on and dims from hd on are 0.  vec: hd and every
+// row's start are multiples of 4 elements.
 template <typename T, int HD>
-__device__ __forceinline__ void sk_tile(const T* base, int64_t rs, int r0, int n, int hd, float* tile) {
-  for (int i = threadIdx.x; i < SK_T * HD; i += SK_THREADS) {
-    const int row = i / HD, d = i % HD;
-    tile[row * (HD + 4) + d] = r0 + row < n && d < hd ? sk_ld(base, (r0 + row) * rs + d) : 0.f;
+struct SkFetch {
+  static constexpr int PIECES = SK_T * HD / 4 / SK_THREADS, PPR = HD / 4;
+  f32x4_t x[PIECES];
+  __device__ __forceinline__ void load(const T* base, int64_t rs, int r0, int n, int hd, bool vec) {
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+      const int i = p * SK_THREADS + threadIdx.x, row = r0 + i / PPR, d = i % PPR * 4;
+      x[p] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      if (row >= n || d >= hd) continue;
+      const T* src = base + row * rs + d;
+      if (!vec) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[p][j] = d + j < hd ? sk_ld(src, j) : 0.f;
+      } else if constexpr (sizeof(T) == 4) {
+        x[p] = *reinterpret_cast<const f32x4_t*>(src);
+      } else {
+        const u32x2_t w = *reinterpret_cast<const u32x2_t*>(src);
+        x[p] = f32x4_t{lo_bf16(w[0]), hi_bf16(w[0]), lo_bf16(w[1]), hi_bf16(w[1])};
+      }
+    }
   }
-}
+  __device__ __forceinline__ void store(float* tile) const {
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+      const int i = p * SK_THREADS + threadIdx.x;
+      *reinterpret_cast<f32x4_t*>(tile + i / PPR * (HD + 4) + i % PPR * 4) = x[p];
+    }
+  }
+};
 
 // Row `row` of a (., hd) matrix as an operand: dims 4 s + kg; 0 where !ok.
 template <typename T, int HD>
@@ -100,12 +125,20 @@ __global__ __launch_bounds__(SK_THREADS) void sk_fwd_kernel(SkParams P) {
   const float sl2 = P.scale * SK_LOG2E;
   const SkTiles tiles = sk_key_tiles(P, off + i0, min(off + min(i0 + SK_T, P.Tq), len) - 1);
   const int n = tiles.count();
+  SkFetch<T, HD> fk, fv;
+  auto fetch = [&](int c) {
+    if (c >= n) return;
+    fk.load(k, P.ks_t, tiles.tile(c) * SK_T, len, P.hd, P.vec);
+    fv.load(v, P.vs_t, tiles.tile(c) * SK_T, len, P.hd, P.vec);
+  };
+  fetch(0);
   for (int c = 0; c < n; ++c) {
     const int s0 = tiles.tile(c) * SK_T;
     __syncthreads();
-    sk_tile<T, HD>(k, P.ks_t, s0, len, P.hd, kt);
-    sk_tile<T, HD>(v, P.vs_t, s0, len, P.hd, vt);
+    fk.store(kt);
+    fv.store(vt);
     __syncthreads();
+    fetch(c + 1);
     f32x4_t st[4];
     float mx = -INFINITY;
 #pragma unroll
@@ -170,12 +203,20 @@ __global__ __launch_bounds__(SK_THREADS) void sk_dq_kernel(SkParams P) {
   for (int dt = 0; dt < HD / 16; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   const SkTiles tiles = sk_key_tiles(P, off + i0, min(off + min(i0 + SK_T, P.Tq), len) - 1);
   const int n = tiles.count();
+  SkFetch<T, HD> fk, fv;
+  auto fetch = [&](int c) {
+    if (c >= n) return;
+    fk.load(k, P.ks_t, tiles.tile(c) * SK_T, len, P.hd, P.vec);
+    fv.load(v, P.vs_t, tiles.tile(c) * SK_T, len, P.hd, P.vec);
+  };
+  fetch(0);
   for (int c = 0; c < n; ++c) {
     const int s0 = tiles.tile(c) * SK_T;
     __syncthreads();
-    sk_tile<T, HD>(k, P.ks_t, s0, len, P.hd, kt);
-    sk_tile<T, HD>(v, P.vs_t, s0, len, P.hd, vt);
+    fk.store(kt);
+    fv.store(vt);
     __syncthreads();
+    fetch(c + 1);
     f32x4_t ds[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -217,18 +258,26 @@ __global__ __launch_bounds__(SK_THREADS, 1) void sk_dkv_kernel(SkParams P, SkSin
   const int q_end = min(P.Tq, len - off), near_hi = sk_near_end(P, S, s0);
   const int i_lo = part < 0 ? max(0, s0 - off) / SK_T * SK_T : near_hi + part * S.span;
   const int i_hi = min(q_end, part < 0 ? near_hi : i_lo + S.span);
+  SkFetch<T, HD> fq, fg;
+  float stat = 0.f;  // threads 0..63: lse of a row, 64..127: D
+  auto fetch = [&](int i0, int hh) {
+    if (i0 >= i_hi) return;
+    const int h = g * G + hh;
+    fq.load(static_cast<const T*>(P.q) + b * P.qs_b + h * P.qs_h, P.qs_t, i0, q_end, P.hd, P.vec);
+    fg.load(static_cast<const T*>(P.dout) + b * P.ds_b + h * P.ds_h, P.ds_t, i0, q_end, P.hd, P.vec);
+    const int i = i0 + (threadIdx.x & 63);
+    if (threadIdx.x < 2 * SK_T && i < q_end)
+      stat = (threadIdx.x < SK_T ? P.lse : P.dd)[(static_cast<int64_t>(b) * P.Hq + h) * P.Tq + i];
+  };
+  fetch(i_lo, 0);
   for (int i0 = i_lo; i0 < i_hi; i0 += SK_T)
     for (int hh = 0; hh < G; ++hh) {
-      const int h = g * G + hh;
       __syncthreads();
-      sk_tile<T, HD>(static_cast<const T*>(P.q) + b * P.qs_b + h * P.qs_h, P.qs_t, i0, q_end, P.hd, qt);
-      sk_tile<T, HD>(static_cast<const T*>(P.dout) + b * P.ds_b + h * P.ds_h, P.ds_t, i0, q_end, P.hd, gt);
-      if (threadIdx.x < 2 * SK_T) {
-        const int i = i0 + (threadIdx.x & 63);
-        const float* src = threadIdx.x < SK_T ? P.lse : P.dd;
-        stats[threadIdx.x] = i < q_end ? src[(static_cast<int64_t>(b) * P.Hq + h) * P.Tq + i] : 0.f;
-      }
+      fq.store(qt);
+      fg.store(gt);
+      if (threadIdx.x < 2 * SK_T) stats[threadIdx.x] = stat;
       __syncthreads();
+      fetch(hh + 1 < G ? i0 : i0 + SK_T, hh + 1 < G ? hh + 1 : 0);
       f32x4_t pw[4], ds[4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -305,6 +354,11 @@ void sk_by_width(int64_t hd, F&& f) {
   else f(std::integral_constant<int, 256>{});
 }
 
+// Whether 4 elements at a time can be read from every row of a (B, H, T, hd) operand.
+bool sk_vec(const void* p, int64_t sb, int64_t sh, int64_t st, int64_t hd, int dtype) {
+  return reinterpret_cast<uintptr_t>(p) % (dtype == FSI_DTYPE_F32 ? 16 : 8) == 0 && (sb | sh | st | hd) % 4 == 0;
+}
+
 int sk_check(const char* what, int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t hd, int64_t window,
              int64_t sinks, int dtype) {
   FSI_CHECK_ARG(dtype == FSI_DTYPE_F32 || dtype == FSI_DTYPE_BF16, FSI_ERR_DTYPE, "%s: dtype %d", what, dtype);
@@ -375,6 +429,7 @@ FSI_API int fsi_sink_attn(const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_
     FSI_HIP_LAUNCH_CHECK("sink_attn");
     return FSI_OK;
   }
+  P.vec = sk_vec(k, ks_b, ks_h, ks_t, head_dim, dtype) && sk_vec(v, vs_b, vs_h, vs_t, head_dim, dtype);
   const dim3 grid(static_cast<unsigned>((Tq + SK_T - 1) / SK_T * Hq), static_cast<unsigned>(B));
   sk_by_width(head_dim, [&](auto w) {
     constexpr int HD = decltype(w)::value;
@@ -440,6 +495,8 @@ FSI_API int fsi_sink_attn_bwd(const void* q, int64_t qs_b, int64_t qs_h, int64_t
     FSI_HIP_LAUNCH_CHECK("sink_attn_bwd");
     return FSI_OK;
   }
+  P.vec = sk_vec(q, qs_b, qs_h, qs_t, head_dim, dtype) && sk_vec(k, ks_b, ks_h, ks_t, head_dim, dtype) &&
+          sk_vec(v, vs_b, vs_h, vs_t, head_dim, dtype) && sk_vec(dout, ds_b, ds_h, ds_t, head_dim, dtype);
   const dim3 gq(static_cast<unsigned>((Tq + SK_T - 1) / SK_T * Hq), static_cast<unsigned>(B));
   const dim3 gkv(static_cast<unsigned>(((Tk + SK_T - 1) / SK_T + S.tiles * S.parts) * Hkv), static_cast<unsigned>(B));
   sk_by_width(head_dim, [&](auto w) {
