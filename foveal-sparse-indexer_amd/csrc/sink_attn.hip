@@ -4,6 +4,7 @@
 // lane, rows 4 kg + j of column r, and step j of the next product takes rows {4 kg + j} as its
 // four contraction indices, so P and dS enter it where they are.
 #include <algorithm>
+#include <type_traits>
 
 #include "sink_attn.h"
 
@@ -80,15 +81,16 @@ __device__ __forceinline__ f32x4_t sk_scores(const float* tile, int t, int r, in
   return s;
 }
 
-// acc[dim][col] += sum over the tile's rows X[row][dim] w[row][col]; w holds rows 16 t + 4 kg + j.
-template <int HD>
-__device__ __forceinline__ void sk_accumulate(const float* tile, int r, int kg, const f32x4_t (&w)[4],
+// acc[dim][col] += sum over NT 16-row parts of the tile from part t0, X[row][dim] w[row][col]; w holds
+// rows 16 (t0 + t) + 4 kg + j.
+template <int HD, int NT>
+__device__ __forceinline__ void sk_accumulate(const float* tile, int t0, int r, int kg, const f32x4_t (&w)[NT],
                                               f32x4_t (&acc)[HD / 16]) {
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float* row = tile + (16 * t + 4 * kg + j) * (HD + 4) + r;
+      const float* row = tile + (16 * (t0 + t) + 4 * kg + j) * (HD + 4) + r;
 #pragma unroll
       for (int dt = 0; dt < HD / 16; ++dt) acc[dt] = mfma4(row[16 * dt], w[t][j], acc[dt]);
     }
@@ -104,15 +106,39 @@ __device__ __forceinline__ void sk_store(T* row, int hd, int kg, const f32x4_t (
       if (16 * dt + 4 * kg + j < hd) sk_st(row + 16 * dt + 4 * kg + j, acc[dt][j] * f);
 }
 
-template <typename T, int HD>
+// SPLIT kernels: the four waves own the same 16 columns and a 16-row part of every tile each, and
+// their sums meet in LDS at the end.  Taken where workgroups of 64 columns would leave CUs without
+// one (rule and figures at sk_split_waves): a quarter of the work behind one another, in four times
+// the workgroups.
+//
+// Sum of the waves' accumulators, each times its wave's factor f, in wave 0.
+template <int HD>
+__device__ __forceinline__ void sk_merge(float* lds, int wave, int lane, float f, f32x4_t (&acc)[HD / 16]) {
+  f32x4_t* slot = reinterpret_cast<f32x4_t*>(lds) + lane;
+  __syncthreads();
+#pragma unroll
+  for (int dt = 0; dt < HD / 16; ++dt) {
+    acc[dt] *= f;
+    if (wave > 0) slot[((wave - 1) * (HD / 16) + dt) * 64] = acc[dt];
+  }
+  __syncthreads();
+  if (wave == 0)
+#pragma unroll
+    for (int dt = 0; dt < HD / 16; ++dt)
+#pragma unroll
+      for (int w = 0; w < 3; ++w) acc[dt] += slot[(w * (HD / 16) + dt) * 64];
+}
+
+template <typename T, int HD, bool SPLIT>
 __global__ __launch_bounds__(SK_THREADS) void sk_fwd_kernel(SkParams P) {
+  constexpr int UN = SPLIT ? 16 : SK_T, NT = SPLIT ? 1 : 4;  // queries of a workgroup, tile parts of a wave
   extern __shared__ __attribute__((aligned(16))) float sk_smem[];
   float *kt = sk_smem, *vt = sk_smem + SK_T * (HD + 4);
   const int h = blockIdx.x % P.Hq, b = blockIdx.y, g = h / (P.Hq / P.Hkv);
-  const int i0 = (gridDim.x / P.Hq - 1 - blockIdx.x / P.Hq) * SK_T;  // most keys first
+  const int i0 = (gridDim.x / P.Hq - 1 - blockIdx.x / P.Hq) * UN;  // most keys first
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kg = lane >> 4;
   const int off = P.Tk - P.Tq, len = sk_length(P, b);
-  const int i = i0 + 16 * wave + r, p = off + i;
+  const int i = i0 + (SPLIT ? 0 : 16 * wave) + r, p = off + i, part = SPLIT ? wave : 0;
   const bool live = i < P.Tq && p < len;
   const T* k = static_cast<const T*>(P.k) + b * P.ks_b + g * P.ks_h;
   const T* v = static_cast<const T*>(P.v) + b * P.vs_b + g * P.vs_h;
@@ -123,7 +149,7 @@ __global__ __launch_bounds__(SK_THREADS) void sk_fwd_kernel(SkParams P) {
   for (int dt = 0; dt < HD / 16; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
   const float sl2 = P.scale * SK_LOG2E;
-  const SkTiles tiles = sk_key_tiles(P, off + i0, min(off + min(i0 + SK_T, P.Tq), len) - 1);
+  const SkTiles tiles = sk_key_tiles(P, off + i0, min(off + min(i0 + UN, P.Tq), len) - 1);
   const int n = tiles.count();
   SkFetch<T, HD> fk, fv;
   auto fetch = [&](int c) {
@@ -139,14 +165,14 @@ __global__ __launch_bounds__(SK_THREADS) void sk_fwd_kernel(SkParams P) {
     fv.store(vt);
     __syncthreads();
     fetch(c + 1);
-    f32x4_t st[4];
+    f32x4_t st[NT];
     float mx = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      st[t] = sk_scores<HD>(kt, t, r, kg, qf);
+    for (int t = 0; t < NT; ++t) {
+      st[t] = sk_scores<HD>(kt, part + t, r, kg, qf);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        st[t][j] = live && sk_visible(P, len, p, s0 + 16 * t + 4 * kg + j) ? st[t][j] * sl2 : -INFINITY;
+        st[t][j] = live && sk_visible(P, len, p, s0 + 16 * (part + t) + 4 * kg + j) ? st[t][j] * sl2 : -INFINITY;
         mx = fmaxf(mx, st[t][j]);
       }
     }
@@ -156,7 +182,7 @@ __global__ __launch_bounds__(SK_THREADS) void sk_fwd_kernel(SkParams P) {
     m = m_new;
     float sum = 0.f;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         st[t][j] = __builtin_amdgcn_exp2f(st[t][j] - ref);
@@ -165,7 +191,25 @@ __global__ __launch_bounds__(SK_THREADS) void sk_fwd_kernel(SkParams P) {
     l = l * alpha + sum_rows4(sum);
 #pragma unroll
     for (int dt = 0; dt < HD / 16; ++dt) acc[dt] *= alpha;
-    sk_accumulate<HD>(vt, r, kg, st, acc);
+    sk_accumulate<HD, NT>(vt, part, r, kg, st, acc);
+  }
+  if constexpr (SPLIT) {  // the waves' maxima and sums, then their accumulators at the common maximum
+    __syncthreads();
+    if (kg == 0) {
+      sk_smem[wave * 32 + r] = m;
+      sk_smem[wave * 32 + 16 + r] = l;
+    }
+    __syncthreads();
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, sk_smem[w * 32 + r]);
+    const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) sum = fmaf(sk_smem[w * 32 + 16 + r], __builtin_amdgcn_exp2f(sk_smem[w * 32 + r] - ref), sum);
+    sk_merge<HD>(sk_smem, wave, lane, __builtin_amdgcn_exp2f(m - ref), acc);
+    m = top;
+    l = sum;
+    if (wave > 0) return;
   }
   if (i >= P.Tq) return;
   sk_store<T, HD>(static_cast<T*>(P.o) + b * P.os_b + h * P.os_h + i * P.os_t, P.hd, kg, acc, l == 0.f ? 0.f : 1.f / l);
@@ -174,15 +218,16 @@ __global__ __launch_bounds__(SK_THREADS) void sk_fwd_kernel(SkParams P) {
 }
 
 // dQ of 16 queries a wave, and D.
-template <typename T, int HD>
+template <typename T, int HD, bool SPLIT>
 __global__ __launch_bounds__(SK_THREADS) void sk_dq_kernel(SkParams P) {
+  constexpr int UN = SPLIT ? 16 : SK_T, NT = SPLIT ? 1 : 4;  // queries of a workgroup, tile parts of a wave
   extern __shared__ __attribute__((aligned(16))) float sk_smem[];
   float *kt = sk_smem, *vt = sk_smem + SK_T * (HD + 4);
   const int h = blockIdx.x % P.Hq, b = blockIdx.y, g = h / (P.Hq / P.Hkv);
-  const int i0 = (gridDim.x / P.Hq - 1 - blockIdx.x / P.Hq) * SK_T;
+  const int i0 = (gridDim.x / P.Hq - 1 - blockIdx.x / P.Hq) * UN;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kg = lane >> 4;
   const int off = P.Tk - P.Tq, len = sk_length(P, b);
-  const int i = i0 + 16 * wave + r, p = off + i;
+  const int i = i0 + (SPLIT ? 0 : 16 * wave) + r, p = off + i, part = SPLIT ? wave : 0;
   const bool live = i < P.Tq && p < len;
   const T* k = static_cast<const T*>(P.k) + b * P.ks_b + g * P.ks_h;
   const T* v = static_cast<const T*>(P.v) + b * P.vs_b + g * P.vs_h;
@@ -196,12 +241,12 @@ __global__ __launch_bounds__(SK_THREADS) void sk_dq_kernel(SkParams P) {
   for (int s = 0; s < HD / 4; ++s)
     if (live && 4 * s + kg < P.hd) dd = fmaf(df[s], sk_ld(o, 4 * s + kg), dd);
   dd = sum_rows4(dd);
-  if (i < P.Tq && kg == 0) P.dd[stat] = dd;
+  if (i < P.Tq && kg == 0 && part == 0) P.dd[stat] = dd;
   const float lse = live ? P.lse[stat] : INFINITY, sl2 = P.scale * SK_LOG2E;
   f32x4_t acc[HD / 16];
 #pragma unroll
   for (int dt = 0; dt < HD / 16; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  const SkTiles tiles = sk_key_tiles(P, off + i0, min(off + min(i0 + SK_T, P.Tq), len) - 1);
+  const SkTiles tiles = sk_key_tiles(P, off + i0, min(off + min(i0 + UN, P.Tq), len) - 1);
   const int n = tiles.count();
   SkFetch<T, HD> fk, fv;
   auto fetch = [&](int c) {
@@ -217,17 +262,21 @@ __global__ __launch_bounds__(SK_THREADS) void sk_dq_kernel(SkParams P) {
     fv.store(vt);
     __syncthreads();
     fetch(c + 1);
-    f32x4_t ds[4];
+    f32x4_t ds[NT];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const f32x4_t s = sk_scores<HD>(kt, t, r, kg, qf), dp = sk_scores<HD>(vt, t, r, kg, df);
+    for (int t = 0; t < NT; ++t) {
+      const f32x4_t s = sk_scores<HD>(kt, part + t, r, kg, qf), dp = sk_scores<HD>(vt, part + t, r, kg, df);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const bool ok = live && sk_visible(P, len, p, s0 + 16 * t + 4 * kg + j);
+        const bool ok = live && sk_visible(P, len, p, s0 + 16 * (part + t) + 4 * kg + j);
         ds[t][j] = ok ? __builtin_amdgcn_exp2f(fmaf(s[j], sl2, -lse)) * (dp[j] - dd) : 0.f;
       }
     }
-    sk_accumulate<HD>(kt, r, kg, ds, acc);
+    sk_accumulate<HD, NT>(kt, part, r, kg, ds, acc);
+  }
+  if constexpr (SPLIT) {
+    sk_merge<HD>(sk_smem, wave, lane, 1.f, acc);
+    if (wave > 0) return;
   }
   if (i < P.Tq)
     sk_store<T, HD>(static_cast<T*>(P.dq) + ((static_cast<int64_t>(b) * P.Hq + h) * P.Tq + i) * P.hd, P.hd, kg, acc,
@@ -235,18 +284,19 @@ __global__ __launch_bounds__(SK_THREADS) void sk_dq_kernel(SkParams P) {
 }
 
 // dK and dV of 16 keys a wave: every query tile that reaches the 64 keys, every query head.
-template <typename T, int HD>
+template <typename T, int HD, bool SPLIT>
 __global__ __launch_bounds__(SK_THREADS, 1) void sk_dkv_kernel(SkParams P, SkSinkSplit S) {
+  constexpr int UN = SPLIT ? 16 : SK_T, NT = SPLIT ? 1 : 4;  // keys of a workgroup, tile parts of a wave
   extern __shared__ __attribute__((aligned(16))) float sk_smem[];
   float *qt = sk_smem, *gt = sk_smem + SK_T * (HD + 4), *stats = sk_smem + 2 * SK_T * (HD + 4);
   const int g = static_cast<int>(blockIdx.x) % P.Hkv, b = blockIdx.y;
   // the parts of the split sink tiles come first: they are the longest
   const int x = static_cast<int>(blockIdx.x) / P.Hkv, n_far = S.tiles * S.parts;
   const int tile = x < n_far ? x / S.parts : x - n_far, part = x < n_far ? x % S.parts : -1;
-  const int s0 = tile * SK_T, G = P.Hq / P.Hkv;
+  const int s0 = tile * UN, G = P.Hq / P.Hkv;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kg = lane >> 4;
   const int off = P.Tk - P.Tq, len = sk_length(P, b);
-  const int s = s0 + 16 * wave + r;
+  const int s = s0 + (SPLIT ? 0 : 16 * wave) + r, tp = SPLIT ? wave : 0;
   float kf[HD / 4], vf[HD / 4];
   sk_frag<T, HD>(static_cast<const T*>(P.k) + b * P.ks_b + g * P.ks_h, P.ks_t, s, s < len, P.hd, kg, kf);
   sk_frag<T, HD>(static_cast<const T*>(P.v) + b * P.vs_b + g * P.vs_h, P.vs_t, s, s < len, P.hd, kg, vf);
@@ -278,21 +328,26 @@ __global__ __launch_bounds__(SK_THREADS, 1) void sk_dkv_kernel(SkParams P, SkSin
       if (threadIdx.x < 2 * SK_T) stats[threadIdx.x] = stat;
       __syncthreads();
       fetch(hh + 1 < G ? i0 : i0 + SK_T, hh + 1 < G ? hh + 1 : 0);
-      f32x4_t pw[4], ds[4];
+      f32x4_t pw[NT], ds[NT];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const f32x4_t sc = sk_scores<HD>(qt, t, r, kg, kf), dp = sk_scores<HD>(gt, t, r, kg, vf);
+      for (int t = 0; t < NT; ++t) {
+        const f32x4_t sc = sk_scores<HD>(qt, tp + t, r, kg, kf), dp = sk_scores<HD>(gt, tp + t, r, kg, vf);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int row = 16 * t + 4 * kg + j, i = i0 + row;
+          const int row = 16 * (tp + t) + 4 * kg + j, i = i0 + row;
           const bool ok = i < q_end && sk_visible(P, len, off + i, s);
           pw[t][j] = ok ? __builtin_amdgcn_exp2f(fmaf(sc[j], sl2, -stats[row])) : 0.f;
           ds[t][j] = ok ? pw[t][j] * (dp[j] - stats[SK_T + row]) : 0.f;
         }
       }
-      sk_accumulate<HD>(gt, r, kg, pw, dv);
-      sk_accumulate<HD>(qt, r, kg, ds, dk);
+      sk_accumulate<HD, NT>(gt, tp, r, kg, pw, dv);
+      sk_accumulate<HD, NT>(qt, tp, r, kg, ds, dk);
     }
+  if constexpr (SPLIT) {
+    sk_merge<HD>(sk_smem, wave, lane, 1.f, dk);
+    sk_merge<HD>(sk_smem, wave, lane, 1.f, dv);
+    if (wave > 0) return;
+  }
   if (s >= P.Tk) return;
   const int64_t head = static_cast<int64_t>(b) * P.Hkv + g;
   if (n_far > 0 && s < P.sinks) {  // a term of the row's sum
@@ -336,6 +391,10 @@ SkSinkSplit sk_split(int64_t Tq, int64_t Tk, int64_t window, int64_t sinks) {
   return S;
 }
 
+// Whether `cols` columns of `heads` (sequence, head) pairs go to SPLIT workgroups: where workgroups
+// of 64 are fewer than the chip's CUs.
+bool sk_split_waves(int64_t cols, int64_t heads) { return (cols + SK_T - 1) / SK_T * heads < 256; }
+
 // LDS above 64 KiB a workgroup has to be asked for.
 template <typename K, typename... A>
 void sk_launch(K* kern, dim3 grid, size_t lds, hipStream_t st, const A&... args) {
@@ -354,6 +413,17 @@ void sk_by_width(int64_t hd, F&& f) {
   else f(std::integral_constant<int, 256>{});
 }
 
+// f(type tag, SPLIT tag).
+template <typename F>
+void sk_by_form(int dtype, bool split, F&& f) {
+  auto by_type = [&](auto t) {
+    if (split) f(t, std::true_type{});
+    else f(t, std::false_type{});
+  };
+  if (dtype == FSI_DTYPE_F32) by_type(float{});
+  else by_type(bf16_t{});
+}
+
 // Whether 4 elements at a time can be read from every row of a (B, H, T, hd) operand.
 bool sk_vec(const void* p, int64_t sb, int64_t sh, int64_t st, int64_t hd, int dtype) {
   return reinterpret_cast<uintptr_t>(p) % (dtype == FSI_DTYPE_F32 ? 16 : 8) == 0 && (sb | sh | st | hd) % 4 == 0;
@@ -368,7 +438,7 @@ int sk_check(const char* what, int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, i
                 (long long)Hq, (long long)Hkv, (long long)Tq, (long long)Tk);
   FSI_CHECK_ARG(window >= 0 && sinks >= 0, FSI_ERR_SHAPE, "%s: window %lld, sinks %lld", what, (long long)window,
                 (long long)sinks);
-  FSI_CHECK_ARG(Tk <= (int64_t(1) << 30) && B <= 65535 && (Tk + SK_T - 1) / SK_T * Hq <= 0x7fffffff, FSI_ERR_SHAPE,
+  FSI_CHECK_ARG(Tk <= (int64_t(1) << 30) && B <= 65535 && (Tk + 15) / 16 * Hq <= 0x7fffffff, FSI_ERR_SHAPE,
                 "%s: sizes beyond range", what);
   return FSI_OK;
 }
@@ -430,12 +500,14 @@ FSI_API int fsi_sink_attn(const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_
     return FSI_OK;
   }
   P.vec = sk_vec(k, ks_b, ks_h, ks_t, head_dim, dtype) && sk_vec(v, vs_b, vs_h, vs_t, head_dim, dtype);
-  const dim3 grid(static_cast<unsigned>((Tq + SK_T - 1) / SK_T * Hq), static_cast<unsigned>(B));
+  auto run = [&](auto t, auto w, auto sp) {
+    using T = decltype(t);
+    constexpr int HD = decltype(w)::value, UN = decltype(sp)::value ? 16 : SK_T;
+    const dim3 grid(static_cast<unsigned>((Tq + UN - 1) / UN * Hq), static_cast<unsigned>(B));
+    sk_launch(&sk_fwd_kernel<T, HD, decltype(sp)::value>, grid, sizeof(float) * 2 * SK_T * (HD + 4), st, P);
+  };
   sk_by_width(head_dim, [&](auto w) {
-    constexpr int HD = decltype(w)::value;
-    const size_t lds = sizeof(float) * 2 * SK_T * (HD + 4);
-    if (dtype == FSI_DTYPE_F32) sk_launch(&sk_fwd_kernel<float, HD>, grid, lds, st, P);
-    else sk_launch(&sk_fwd_kernel<bf16_t, HD>, grid, lds, st, P);
+    sk_by_form(dtype, sk_split_waves(Tq, B * Hq), [&](auto t, auto sp) { run(t, w, sp); });
   });
   FSI_HIP_LAUNCH_CHECK("sink_attn");
   return FSI_OK;
@@ -478,7 +550,7 @@ FSI_API int fsi_sink_attn_bwd(const void* q, int64_t qs_b, int64_t qs_h, int64_t
   P.dv = dv;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   SkSinkSplit S = sk_split(Tq, Tk, window, sinks);
-  FSI_CHECK_ARG(B * Hkv * P.sinks <= 0x7fffffff && ((Tk + SK_T - 1) / SK_T + S.tiles * S.parts) * Hkv <= 0x7fffffff,
+  FSI_CHECK_ARG(B * Hkv * P.sinks <= 0x7fffffff && ((Tk + 15) / 16 + 4 * S.tiles * S.parts) * Hkv <= 0x7fffffff,
                 FSI_ERR_SHAPE, "sink_attn_bwd: sizes beyond range");
   if (S.parts)
     S.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) +
@@ -497,18 +569,25 @@ FSI_API int fsi_sink_attn_bwd(const void* q, int64_t qs_b, int64_t qs_h, int64_t
   }
   P.vec = sk_vec(q, qs_b, qs_h, qs_t, head_dim, dtype) && sk_vec(k, ks_b, ks_h, ks_t, head_dim, dtype) &&
           sk_vec(v, vs_b, vs_h, vs_t, head_dim, dtype) && sk_vec(dout, ds_b, ds_h, ds_t, head_dim, dtype);
-  const dim3 gq(static_cast<unsigned>((Tq + SK_T - 1) / SK_T * Hq), static_cast<unsigned>(B));
-  const dim3 gkv(static_cast<unsigned>(((Tk + SK_T - 1) / SK_T + S.tiles * S.parts) * Hkv), static_cast<unsigned>(B));
+  auto run_q = [&](auto t, auto w, auto sp) {
+    using T = decltype(t);
+    constexpr int HD = decltype(w)::value, UN = decltype(sp)::value ? 16 : SK_T;
+    const dim3 grid(static_cast<unsigned>((Tq + UN - 1) / UN * Hq), static_cast<unsigned>(B));
+    sk_launch(&sk_dq_kernel<T, HD, decltype(sp)::value>, grid, sizeof(float) * 2 * SK_T * (HD + 4), st, P);
+  };
+  auto run_kv = [&](auto t, auto w, auto sp) {
+    using T = decltype(t);
+    constexpr int HD = decltype(w)::value, UN = decltype(sp)::value ? 16 : SK_T;
+    SkSinkSplit SU = S;
+    if (S.parts) SU.tiles = (P.sinks + UN - 1) / UN;
+    const dim3 grid(static_cast<unsigned>(((Tk + UN - 1) / UN + SU.tiles * SU.parts) * Hkv), static_cast<unsigned>(B));
+    sk_launch(&sk_dkv_kernel<T, HD, decltype(sp)::value>, grid, sizeof(float) * (2 * SK_T * (HD + 4) + 2 * SK_T), st, P,
+              SU);
+  };
   sk_by_width(head_dim, [&](auto w) {
-    constexpr int HD = decltype(w)::value;
-    const size_t lds = sizeof(float) * 2 * SK_T * (HD + 4), lds_kv = lds + sizeof(float) * 2 * SK_T;
-    if (dtype == FSI_DTYPE_F32) {
-      if (Tq > 0) sk_launch(&sk_dq_kernel<float, HD>, gq, lds, st, P);
-      sk_launch(&sk_dkv_kernel<float, HD>, gkv, lds_kv, st, P, S);
-    } else {
-      if (Tq > 0) sk_launch(&sk_dq_kernel<bf16_t, HD>, gq, lds, st, P);
-      sk_launch(&sk_dkv_kernel<bf16_t, HD>, gkv, lds_kv, st, P, S);
-    }
+    if (Tq > 0)
+      sk_by_form(dtype, sk_split_waves(Tq, B * Hq), [&](auto t, auto sp) { run_q(t, w, sp); });
+    sk_by_form(dtype, sk_split_waves(Tk, B * Hkv), [&](auto t, auto sp) { run_kv(t, w, sp); });
   });
   sum_sinks();
   FSI_HIP_LAUNCH_CHECK("sink_attn_bwd");
