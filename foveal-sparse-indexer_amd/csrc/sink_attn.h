@@ -33,6 +33,14 @@ struct SkParams {
   void* dq;    // contiguous gradients of the operands' type
   void* dk;
   void* dv;
+  // Key tiles of a query block cut into ksplit workgroups (forward, dQ): fp32 rows of
+  // sk_part_stride(hd) floats, (ksplit, B, Hq, Tq), that sk_join_kernel combines.
+  int ksplit;
+  float* kpart;
+  // Query heads of a KV head cut into hsplit workgroups (dK, dV): fp32 rows (hsplit, B, Hkv, Tk, [dK,
+  // dV], hd), added by sk_kv_sum_kernel.
+  int hsplit;
+  float* hpart;
   bool vec;    // sink_attn.hip's kernels: 4 elements at a time can be read from the tiles' rows
 };
 
@@ -59,19 +67,52 @@ __device__ __forceinline__ SkTiles sk_key_tiles(const SkParams& P, int p0, int p
   return t;
 }
 
-__device__ __forceinline__ bool sk_visible(const SkParams& P, int len, int p, int s) {
-  return s <= p && (s > p - P.window || s < P.sinks) && p < len;
-}
-
 // A tile of sink keys is seen by every later query, far more than a window's: its queries beyond
 // the window are cut into `parts` of `span` queries (a multiple of the tile), each a workgroup of
-// its own that leaves fp32 sums of the sink rows in `sums` (B, Hkv, parts + 1, sinks, [dK, dV], hd),
-// the window's own queries as the last part; sk_sink_sum_kernel adds them in that order.
+// its own that leaves fp32 sums of the sink rows in `sums` (B, Hkv, hsplit, parts + 1, sinks, [dK, dV],
+// hd), the window's own queries as the last part; sk_kv_sum_kernel adds them in that order.
 // parts 0: no such split, a sink tile's workgroup takes all of its queries.
 struct SkSinkSplit {
   int tiles, parts, span;
   float* sums;
 };
+
+// A partial row: the accumulated dims, then (forward) the maximum, the sum that divides the output and
+// the sum that makes lse.
+__host__ __device__ __forceinline__ int sk_part_stride(int hd) { return (hd + 3) / 4 * 4 + 4; }
+__device__ __forceinline__ float* sk_part_row(const SkParams& P, int z, int b, int h, int i) {
+  return P.kpart + (((static_cast<int64_t>(z) * P.B + b) * P.Hq + h) * P.Tq + i) * sk_part_stride(P.hd);
+}
+
+// Tiles [lo, hi) of part z of a query block's n key tiles.
+struct SkRange {
+  int lo, hi;
+};
+__device__ __forceinline__ SkRange sk_key_part(const SkParams& P, int n, int z) {
+  const int per = (n + P.ksplit - 1) / P.ksplit, lo = min(n, z * per);
+  return {lo, min(n, lo + per)};
+}
+// Query heads [lo, hi) of part z of a KV head's group.
+__device__ __forceinline__ SkRange sk_head_part(const SkParams& P, int z) {
+  const int G = P.Hq / P.Hkv, per = (G + P.hsplit - 1) / P.hsplit, lo = min(G, z * per);
+  return {lo, min(G, lo + per)};
+}
+
+// Where key row s of (b, g) goes to as fp32 (dK, then dV at + hd): a term of a split sum, or null for
+// a row that is stored as it is.  far: the part of a split sink tile (-1: the window's queries).
+__device__ __forceinline__ float* sk_kv_term(const SkParams& P, const SkSinkSplit& S, int64_t head, int s, int z,
+                                             int far) {
+  if (S.parts > 0 && s < P.sinks)
+    return S.sums +
+           ((((head * P.hsplit + z) * (S.parts + 1) + (far < 0 ? S.parts : far)) * P.sinks + s) * 2) * P.hd;
+  if (P.hsplit == 1) return nullptr;
+  const int64_t heads = static_cast<int64_t>(P.B) * P.Hkv;
+  return P.hpart + (((z * heads + head) * P.Tk + s) * 2) * P.hd;
+}
+
+__device__ __forceinline__ bool sk_visible(const SkParams& P, int len, int p, int s) {
+  return s <= p && (s > p - P.window || s < P.sinks) && p < len;
+}
 
 // End of the queries that reach key tile s0 before the split's parts begin, in whole query tiles.
 __device__ __forceinline__ int sk_near_end(const SkParams& P, const SkSinkSplit& S, int s0) {
@@ -82,7 +123,9 @@ __device__ __forceinline__ int sk_near_end(const SkParams& P, const SkSinkSplit&
 }
 
 // The bf16 kernels of sink_attn_bf16.hip: whether they take the call, and their launches.
+// sb_query_blocks: the workgroups of the forward (dQ) without a split of the keys.
 bool sb_takes(const SkParams& P, int dtype, bool backward);
+int64_t sb_query_blocks(const SkParams& P, bool backward);
 void sb_forward(const SkParams& P, hipStream_t st);
 void sb_backward(const SkParams& P, const SkSinkSplit& S, hipStream_t st);
 

@@ -150,15 +150,15 @@ __global__ __launch_bounds__(SK_THREADS) void sk_fwd_kernel(SkParams P) {
   float m = -INFINITY, l = 0.f;
   const float sl2 = P.scale * SK_LOG2E;
   const SkTiles tiles = sk_key_tiles(P, off + i0, min(off + min(i0 + UN, P.Tq), len) - 1);
-  const int n = tiles.count();
+  const SkRange range = sk_key_part(P, tiles.count(), blockIdx.z);
   SkFetch<T, HD> fk, fv;
   auto fetch = [&](int c) {
-    if (c >= n) return;
+    if (c >= range.hi) return;
     fk.load(k, P.ks_t, tiles.tile(c) * SK_T, len, P.hd, P.vec);
     fv.load(v, P.vs_t, tiles.tile(c) * SK_T, len, P.hd, P.vec);
   };
-  fetch(0);
-  for (int c = 0; c < n; ++c) {
+  fetch(range.lo);
+  for (int c = range.lo; c < range.hi; ++c) {
     const int s0 = tiles.tile(c) * SK_T;
     __syncthreads();
     fk.store(kt);
@@ -212,6 +212,12 @@ __global__ __launch_bounds__(SK_THREADS) void sk_fwd_kernel(SkParams P) {
     if (wave > 0) return;
   }
   if (i >= P.Tq) return;
+  if (P.ksplit > 1) {
+    float* row = sk_part_row(P, blockIdx.z, b, h, i);
+    sk_store<float, HD>(row, P.hd, kg, acc, 1.f);
+    if (kg == 0) *reinterpret_cast<f32x4_t*>(row + sk_part_stride(P.hd) - 4) = f32x4_t{m, l, l, 0.f};
+    return;
+  }
   sk_store<T, HD>(static_cast<T*>(P.o) + b * P.os_b + h * P.os_h + i * P.os_t, P.hd, kg, acc, l == 0.f ? 0.f : 1.f / l);
   if (P.lse && kg == 0)
     P.lse[(static_cast<int64_t>(b) * P.Hq + h) * P.Tq + i] = l == 0.f ? INFINITY : m + __log2f(l);
@@ -241,21 +247,21 @@ __global__ __launch_bounds__(SK_THREADS) void sk_dq_kernel(SkParams P) {
   for (int s = 0; s < HD / 4; ++s)
     if (live && 4 * s + kg < P.hd) dd = fmaf(df[s], sk_ld(o, 4 * s + kg), dd);
   dd = sum_rows4(dd);
-  if (i < P.Tq && kg == 0 && part == 0) P.dd[stat] = dd;
+  if (i < P.Tq && kg == 0 && part == 0 && blockIdx.z == 0) P.dd[stat] = dd;
   const float lse = live ? P.lse[stat] : INFINITY, sl2 = P.scale * SK_LOG2E;
   f32x4_t acc[HD / 16];
 #pragma unroll
   for (int dt = 0; dt < HD / 16; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   const SkTiles tiles = sk_key_tiles(P, off + i0, min(off + min(i0 + UN, P.Tq), len) - 1);
-  const int n = tiles.count();
+  const SkRange range = sk_key_part(P, tiles.count(), blockIdx.z);
   SkFetch<T, HD> fk, fv;
   auto fetch = [&](int c) {
-    if (c >= n) return;
+    if (c >= range.hi) return;
     fk.load(k, P.ks_t, tiles.tile(c) * SK_T, len, P.hd, P.vec);
     fv.load(v, P.vs_t, tiles.tile(c) * SK_T, len, P.hd, P.vec);
   };
-  fetch(0);
-  for (int c = 0; c < n; ++c) {
+  fetch(range.lo);
+  for (int c = range.lo; c < range.hi; ++c) {
     const int s0 = tiles.tile(c) * SK_T;
     __syncthreads();
     fk.store(kt);
@@ -278,7 +284,10 @@ __global__ __launch_bounds__(SK_THREADS) void sk_dq_kernel(SkParams P) {
     sk_merge<HD>(sk_smem, wave, lane, 1.f, acc);
     if (wave > 0) return;
   }
-  if (i < P.Tq)
+  if (i >= P.Tq) return;
+  if (P.ksplit > 1)
+    sk_store<float, HD>(sk_part_row(P, blockIdx.z, b, h, i), P.hd, kg, acc, P.scale);
+  else
     sk_store<T, HD>(static_cast<T*>(P.dq) + ((static_cast<int64_t>(b) * P.Hq + h) * P.Tq + i) * P.hd, P.hd, kg, acc,
                     P.scale);
 }
@@ -294,6 +303,7 @@ __global__ __launch_bounds__(SK_THREADS, 1) void sk_dkv_kernel(SkParams P, SkSin
   const int x = static_cast<int>(blockIdx.x) / P.Hkv, n_far = S.tiles * S.parts;
   const int tile = x < n_far ? x / S.parts : x - n_far, part = x < n_far ? x % S.parts : -1;
   const int s0 = tile * UN, G = P.Hq / P.Hkv;
+  const SkRange heads = sk_head_part(P, blockIdx.z);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kg = lane >> 4;
   const int off = P.Tk - P.Tq, len = sk_length(P, b);
   const int s = s0 + (SPLIT ? 0 : 16 * wave) + r, tp = SPLIT ? wave : 0;
@@ -311,7 +321,7 @@ __global__ __launch_bounds__(SK_THREADS, 1) void sk_dkv_kernel(SkParams P, SkSin
   SkFetch<T, HD> fq, fg;
   float stat = 0.f;  // threads 0..63: lse of a row, 64..127: D
   auto fetch = [&](int i0, int hh) {
-    if (i0 >= i_hi) return;
+    if (i0 >= i_hi || hh >= heads.hi) return;
     const int h = g * G + hh;
     fq.load(static_cast<const T*>(P.q) + b * P.qs_b + h * P.qs_h, P.qs_t, i0, q_end, P.hd, P.vec);
     fg.load(static_cast<const T*>(P.dout) + b * P.ds_b + h * P.ds_h, P.ds_t, i0, q_end, P.hd, P.vec);
@@ -319,15 +329,15 @@ __global__ __launch_bounds__(SK_THREADS, 1) void sk_dkv_kernel(SkParams P, SkSin
     if (threadIdx.x < 2 * SK_T && i < q_end)
       stat = (threadIdx.x < SK_T ? P.lse : P.dd)[(static_cast<int64_t>(b) * P.Hq + h) * P.Tq + i];
   };
-  fetch(i_lo, 0);
+  fetch(i_lo, heads.lo);
   for (int i0 = i_lo; i0 < i_hi; i0 += SK_T)
-    for (int hh = 0; hh < G; ++hh) {
+    for (int hh = heads.lo; hh < heads.hi; ++hh) {
       __syncthreads();
       fq.store(qt);
       fg.store(gt);
       if (threadIdx.x < 2 * SK_T) stats[threadIdx.x] = stat;
       __syncthreads();
-      fetch(hh + 1 < G ? i0 : i0 + SK_T, hh + 1 < G ? hh + 1 : 0);
+      fetch(hh + 1 < heads.hi ? i0 : i0 + SK_T, hh + 1 < heads.hi ? hh + 1 : heads.lo);
       f32x4_t pw[NT], ds[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
@@ -350,8 +360,8 @@ __global__ __launch_bounds__(SK_THREADS, 1) void sk_dkv_kernel(SkParams P, SkSin
   }
   if (s >= P.Tk) return;
   const int64_t head = static_cast<int64_t>(b) * P.Hkv + g;
-  if (n_far > 0 && s < P.sinks) {  // a term of the row's sum
-    float* t = S.sums + (((head * (S.parts + 1) + (part < 0 ? S.parts : part)) * P.sinks + s) * 2) * P.hd;
+  if (float* t = sk_kv_term(P, S, head, s, blockIdx.z, part)) {
+    if (part >= 0 && s >= P.sinks) return;
     sk_store<float, HD>(t, P.hd, kg, dk, P.scale);
     sk_store<float, HD>(t + P.hd, P.hd, kg, dv, 1.f);
   } else if (part < 0) {
@@ -361,17 +371,50 @@ __global__ __launch_bounds__(SK_THREADS, 1) void sk_dkv_kernel(SkParams P, SkSin
   }
 }
 
-// dK and dV rows of split sink tiles: the parts' sums in order, one workgroup per (head, sink).
+// dK and dV rows that come in terms (sk_kv_term), added in order: one workgroup per (head, row); the
+// first `rows` rows of every head.
 template <typename T>
-__global__ __launch_bounds__(SK_THREADS) void sk_sink_sum_kernel(SkParams P, SkSinkSplit S) {
-  const int s = static_cast<int>(blockIdx.x) % P.sinks;
-  const int64_t head = blockIdx.x / P.sinks;
+__global__ __launch_bounds__(SK_THREADS) void sk_kv_sum_kernel(SkParams P, SkSinkSplit S, int rows) {
+  const int s = static_cast<int>(blockIdx.x % rows);
+  const int64_t head = blockIdx.x / rows;
+  const int far = S.parts > 0 && s < P.sinks ? S.parts + 1 : 1;
   for (int d = threadIdx.x; d < 2 * P.hd; d += SK_THREADS) {
     float sum = 0.f;
-    for (int part = 0; part <= S.parts; ++part)
-      sum += S.sums[((head * (S.parts + 1) + part) * P.sinks + s) * 2 * P.hd + d];
+    for (int z = 0; z < P.hsplit; ++z)
+      for (int part = 0; part < far; ++part) sum += sk_kv_term(P, S, head, s, z, far > 1 && part < S.parts ? part : -1)[d];
     T* out = static_cast<T*>(d < P.hd ? P.dk : P.dv) + (head * P.Tk + s) * P.hd + (d < P.hd ? d : d - P.hd);
     sk_st(out, sum);
+  }
+}
+
+// Output rows from the parts of their keys, one wave per (sequence, head, query): forward (out, lse),
+// or dQ.
+template <typename T, bool FWD>
+__global__ __launch_bounds__(64) void sk_join_kernel(SkParams P) {
+  const int64_t row = blockIdx.x;
+  const int i = static_cast<int>(row % P.Tq), h = static_cast<int>(row / P.Tq % P.Hq);
+  const int b = static_cast<int>(row / P.Tq / P.Hq), last = sk_part_stride(P.hd) - 4;
+  float m = -INFINITY, l = 0.f, lf = 0.f;
+  if constexpr (FWD) {
+    for (int z = 0; z < P.ksplit; ++z) m = fmaxf(m, sk_part_row(P, z, b, h, i)[last]);
+    const float ref = m == -INFINITY ? 0.f : m;
+    for (int z = 0; z < P.ksplit; ++z) {
+      const f32x4_t st = *reinterpret_cast<const f32x4_t*>(sk_part_row(P, z, b, h, i) + last);
+      const float w = __builtin_amdgcn_exp2f(st[0] - ref);
+      l = fmaf(st[1], w, l);
+      lf = fmaf(st[2], w, lf);
+    }
+    if (P.lse && threadIdx.x == 0) P.lse[row] = l == 0.f ? INFINITY : m + __log2f(lf);
+  }
+  const float ref = m == -INFINITY ? 0.f : m, inv = l == 0.f ? 0.f : 1.f / l;
+  for (int d = threadIdx.x; d < P.hd; d += 64) {
+    float x = 0.f;
+    for (int z = 0; z < P.ksplit; ++z) {
+      const float* p = sk_part_row(P, z, b, h, i);
+      x = FWD ? fmaf(p[d], __builtin_amdgcn_exp2f(p[last] - ref), x) : x + p[d];
+    }
+    if constexpr (FWD) sk_st(static_cast<T*>(P.o) + b * P.os_b + h * P.os_h + i * P.os_t + d, x * inv);
+    else sk_st(static_cast<T*>(P.dq) + row * P.hd + d, x);
   }
 }
 
@@ -395,6 +438,56 @@ SkSinkSplit sk_split(int64_t Tq, int64_t Tk, int64_t window, int64_t sinks) {
 // of 64 are fewer than the chip's CUs.
 bool sk_split_waves(int64_t cols, int64_t heads) { return (cols + SK_T - 1) / SK_T * heads < 256; }
 
+// Parts that the keys of `blocks` workgroups are cut into: as many as two workgroups a CU hold, each
+// of 4 key tiles at least.
+constexpr int64_t SK_SLOTS = 512;
+int sk_key_splits(const SkParams& P, int64_t blocks, int64_t columns) {
+  const int64_t span = std::min<int64_t>(P.Tk, static_cast<int64_t>(P.window) + columns);
+  const int64_t tiles = (span + SK_T - 1) / SK_T + 1 + (P.sinks + SK_T - 1) / SK_T;
+  return static_cast<int>(std::max<int64_t>(std::min(SK_SLOTS / std::max<int64_t>(blocks, 1), tiles / 4), 1));
+}
+// Workgroups of the fp32 kernels' forward (dQ), and their queries.
+int64_t sk_query_blocks(const SkParams& P) {
+  const int64_t heads = static_cast<int64_t>(P.B) * P.Hq;
+  return (P.Tq + (sk_split_waves(P.Tq, heads) ? 15 : 63)) / (sk_split_waves(P.Tq, heads) ? 16 : 64) * heads;
+}
+size_t sk_part_bytes(const SkParams& P, int splits) {
+  return splits > 1 ? fsi_host::align_up(sizeof(float) * static_cast<size_t>(splits) * P.B * P.Hq * P.Tq *
+                                             sk_part_stride(P.hd),
+                                         256)
+                    : 0;
+}
+// Parts that the query heads of a KV head are cut into for dK and dV: while the key tiles leave CUs
+// without a workgroup.  unit: keys of a workgroup.
+int sk_head_splits(const SkParams& P, const SkSinkSplit& S, int64_t unit, int64_t slots) {
+  const int64_t far = S.parts ? (P.sinks + unit - 1) / unit * S.parts : 0;
+  const int64_t blocks = ((P.Tk + unit - 1) / unit + far) * P.Hkv * P.B;
+  return static_cast<int>(std::max<int64_t>(std::min<int64_t>(slots / blocks, P.Hq / P.Hkv), 1));
+}
+size_t sk_head_bytes(const SkParams& P, int splits) {
+  return splits > 1 ? fsi_host::align_up(sizeof(float) * 2 * static_cast<size_t>(splits) * P.B * P.Hkv * P.Tk * P.hd, 256)
+                    : 0;
+}
+size_t sk_sums_bytes(const SkParams& P, const SkSinkSplit& S, int hsplit) {
+  return S.parts ? fsi_host::align_up(sizeof(float) * 2 * static_cast<size_t>(hsplit) * P.B * P.Hkv * (S.parts + 1) *
+                                          P.sinks * P.hd,
+                                      256)
+                 : 0;
+}
+// How a backward is cut, for the bf16 kernels or the fp32 ones.
+struct SkPlan {
+  int ksplit, hsplit;
+  size_t bytes(const SkParams& P, const SkSinkSplit& S) const {
+    return fsi_host::align_up(sizeof(float) * static_cast<size_t>(P.B) * P.Hq * P.Tq, 256) + sk_part_bytes(P, ksplit) +
+           sk_head_bytes(P, hsplit) + sk_sums_bytes(P, S, hsplit);
+  }
+};
+SkPlan sk_plan(const SkParams& P, const SkSinkSplit& S, bool bf16) {
+  if (bf16) return {sk_key_splits(P, sb_query_blocks(P, true), 2 * SK_T), sk_head_splits(P, S, SK_T, SK_SLOTS)};
+  return {sk_key_splits(P, sk_query_blocks(P), SK_T),
+          sk_head_splits(P, S, sk_split_waves(P.Tk, static_cast<int64_t>(P.B) * P.Hkv) ? 16 : SK_T, SK_SLOTS / 2)};
+}
+
 // LDS above 64 KiB a workgroup has to be asked for.
 template <typename K, typename... A>
 void sk_launch(K* kern, dim3 grid, size_t lds, hipStream_t st, const A&... args) {
@@ -411,6 +504,14 @@ void sk_by_width(int64_t hd, F&& f) {
   else if (hd <= 96) f(std::integral_constant<int, 96>{});
   else if (hd <= 128) f(std::integral_constant<int, 128>{});
   else f(std::integral_constant<int, 256>{});
+}
+
+template <bool FWD>
+void sk_join(const SkParams& P, int dtype, hipStream_t st) {
+  if (P.ksplit == 1) return;
+  const unsigned rows = static_cast<unsigned>(static_cast<int64_t>(P.B) * P.Hq * P.Tq);
+  if (dtype == FSI_DTYPE_F32) sk_join_kernel<float, FWD><<<rows, 64, 0, st>>>(P);
+  else sk_join_kernel<bf16_t, FWD><<<rows, 64, 0, st>>>(P);
 }
 
 // f(type tag, SPLIT tag).
@@ -475,6 +576,7 @@ SkParams sk_params(const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_t, cons
   P.sinks = (int)std::min<int64_t>(sinks, Tk);
   P.lengths = lengths;
   P.scale = scale;
+  P.ksplit = P.hsplit = 1;
   return P;
 }
 
@@ -482,44 +584,64 @@ SkParams sk_params(const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_t, cons
 
 extern "C" {
 
+FSI_API size_t fsi_sink_attn_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t Tk,
+                                            int64_t head_dim, int64_t window, int64_t sinks) {
+  if (sk_check("sink_attn", B, Hq, Hkv, Tq, Tk, head_dim, window, sinks, FSI_DTYPE_F32) != FSI_OK || B == 0 || Tq == 0)
+    return 0;
+  const SkParams P = sk_params(nullptr, 0, 0, 0, nullptr, 0, 0, 0, nullptr, 0, 0, 0, nullptr, 0, 0, 0, B, Hq, Hkv, Tq,
+                               Tk, head_dim, window, sinks, nullptr, 1.f);
+  return std::max(sk_part_bytes(P, sk_key_splits(P, sk_query_blocks(P), SK_T)),
+                  sk_part_bytes(P, sk_key_splits(P, sb_query_blocks(P, false), 2 * SK_T)));
+}
+
 FSI_API int fsi_sink_attn(const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_t, const void* k, int64_t ks_b,
                           int64_t ks_h, int64_t ks_t, const void* v, int64_t vs_b, int64_t vs_h, int64_t vs_t,
                           int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t head_dim, int64_t window,
                           int64_t sinks, const int32_t* lengths, float scale, int dtype, void* out, int64_t os_b,
-                          int64_t os_h, int64_t os_t, float* lse, void* stream) {
+                          int64_t os_h, int64_t os_t, float* lse, void* workspace, size_t workspace_bytes,
+                          void* stream) {
+  using namespace fsi_host;
   const int c = sk_check("sink_attn", B, Hq, Hkv, Tq, Tk, head_dim, window, sinks, dtype);
   if (c != FSI_OK || B == 0 || Tq == 0) return c;
   FSI_CHECK_ARG(q && k && v && out, FSI_ERR_INVALID_ARG, "sink_attn: null pointer");
+  const size_t need = fsi_sink_attn_workspace_size(B, Hq, Hkv, Tq, Tk, head_dim, window, sinks);
+  FSI_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+                FSI_ERR_WORKSPACE, "sink_attn: workspace %zu < %zu bytes (or misaligned)", workspace_bytes, need);
   SkParams P = sk_params(q, qs_b, qs_h, qs_t, k, ks_b, ks_h, ks_t, v, vs_b, vs_h, vs_t, out, os_b, os_h, os_t, B, Hq,
                          Hkv, Tq, Tk, head_dim, window, sinks, lengths, scale);
   P.lse = lse;
+  P.kpart = static_cast<float*>(workspace);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (sb_takes(P, dtype, false)) {
+    P.ksplit = sk_key_splits(P, sb_query_blocks(P, false), 2 * SK_T);
     sb_forward(P, st);
-    FSI_HIP_LAUNCH_CHECK("sink_attn");
-    return FSI_OK;
+  } else {
+    P.ksplit = sk_key_splits(P, sk_query_blocks(P), SK_T);
+    P.vec = sk_vec(k, ks_b, ks_h, ks_t, head_dim, dtype) && sk_vec(v, vs_b, vs_h, vs_t, head_dim, dtype);
+    auto run = [&](auto t, auto w, auto sp) {
+      using T = decltype(t);
+      constexpr int HD = decltype(w)::value, UN = decltype(sp)::value ? 16 : SK_T;
+      const dim3 grid(static_cast<unsigned>((Tq + UN - 1) / UN * Hq), static_cast<unsigned>(B), P.ksplit);
+      sk_launch(&sk_fwd_kernel<T, HD, decltype(sp)::value>, grid, sizeof(float) * 2 * SK_T * (HD + 4), st, P);
+    };
+    sk_by_width(head_dim, [&](auto w) {
+      sk_by_form(dtype, sk_split_waves(Tq, B * Hq), [&](auto t, auto sp) { run(t, w, sp); });
+    });
   }
-  P.vec = sk_vec(k, ks_b, ks_h, ks_t, head_dim, dtype) && sk_vec(v, vs_b, vs_h, vs_t, head_dim, dtype);
-  auto run = [&](auto t, auto w, auto sp) {
-    using T = decltype(t);
-    constexpr int HD = decltype(w)::value, UN = decltype(sp)::value ? 16 : SK_T;
-    const dim3 grid(static_cast<unsigned>((Tq + UN - 1) / UN * Hq), static_cast<unsigned>(B));
-    sk_launch(&sk_fwd_kernel<T, HD, decltype(sp)::value>, grid, sizeof(float) * 2 * SK_T * (HD + 4), st, P);
-  };
-  sk_by_width(head_dim, [&](auto w) {
-    sk_by_form(dtype, sk_split_waves(Tq, B * Hq), [&](auto t, auto sp) { run(t, w, sp); });
-  });
+  sk_join<true>(P, dtype, st);
   FSI_HIP_LAUNCH_CHECK("sink_attn");
   return FSI_OK;
 }
 
 FSI_API size_t fsi_sink_attn_bwd_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t Tk,
                                                 int64_t head_dim, int64_t window, int64_t sinks) {
-  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Tq <= 0 || Tk < Tq || head_dim <= 0 || window < 0 || sinks < 0) return 0;
+  if (sk_check("sink_attn_bwd", B, Hq, Hkv, Tq, Tk, head_dim, window, sinks, FSI_DTYPE_F32) != FSI_OK || B == 0 ||
+      Tq == 0)
+    return 0;
+  const SkParams P = sk_params(nullptr, 0, 0, 0, nullptr, 0, 0, 0, nullptr, 0, 0, 0, nullptr, 0, 0, 0, B, Hq, Hkv, Tq,
+                               Tk, head_dim, window, sinks, nullptr, 1.f);
   const SkSinkSplit S = sk_split(Tq, Tk, window, sinks);
-  // D of every query, then the split sink tiles' sums
-  return fsi_host::align_up(sizeof(float) * static_cast<size_t>(B * Hq * Tq), 256) +
-         (S.parts ? sizeof(float) * static_cast<size_t>(B * Hkv * (S.parts + 1) * std::min(sinks, Tk) * 2 * head_dim) : 0);
+  return std::max(sk_plan(P, S, false).bytes(P, S), sk_plan(P, S, true).bytes(P, S));
 }
 
 FSI_API int fsi_sink_attn_bwd(const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_t, const void* k, int64_t ks_b,
@@ -544,52 +666,60 @@ FSI_API int fsi_sink_attn_bwd(const void* q, int64_t qs_b, int64_t qs_h, int64_t
   P.ds_h = ds_h;
   P.ds_t = ds_t;
   P.lse = const_cast<float*>(lse);
-  P.dd = static_cast<float*>(workspace);
   P.dq = dq;
   P.dk = dk;
   P.dv = dv;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   SkSinkSplit S = sk_split(Tq, Tk, window, sinks);
-  FSI_CHECK_ARG(B * Hkv * P.sinks <= 0x7fffffff && ((Tk + 15) / 16 + 4 * S.tiles * S.parts) * Hkv <= 0x7fffffff,
+  FSI_CHECK_ARG(B * Hkv * Tk <= 0x7fffffff && ((Tk + 15) / 16 + 4 * S.tiles * S.parts) * Hkv <= 0x7fffffff,
                 FSI_ERR_SHAPE, "sink_attn_bwd: sizes beyond range");
-  if (S.parts)
-    S.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                      align_up(sizeof(float) * static_cast<size_t>(B * Hq * Tq), 256));
-  auto sum_sinks = [&] {
-    if (!S.parts) return;
-    const unsigned rows = static_cast<unsigned>(B * Hkv * P.sinks);
-    if (dtype == FSI_DTYPE_F32) sk_sink_sum_kernel<float><<<rows, SK_THREADS, 0, st>>>(P, S);
-    else sk_sink_sum_kernel<bf16_t><<<rows, SK_THREADS, 0, st>>>(P, S);
-  };
-  if (sb_takes(P, dtype, true)) {
-    sb_backward(P, S, st);
-    sum_sinks();
-    FSI_HIP_LAUNCH_CHECK("sink_attn_bwd");
-    return FSI_OK;
+  const bool bf16 = sb_takes(P, dtype, true);
+  if (Tq > 0) {  // D, the parts of dQ, of dK / dV, and of the sink rows
+    const SkPlan plan = sk_plan(P, S, bf16);
+    P.ksplit = plan.ksplit;
+    P.hsplit = plan.hsplit;
+    char* ws = static_cast<char*>(workspace);
+    P.dd = reinterpret_cast<float*>(ws);
+    ws += align_up(sizeof(float) * static_cast<size_t>(B * Hq * Tq), 256);
+    P.kpart = reinterpret_cast<float*>(ws);
+    ws += sk_part_bytes(P, P.ksplit);
+    P.hpart = reinterpret_cast<float*>(ws);
+    ws += sk_head_bytes(P, P.hsplit);
+    S.sums = reinterpret_cast<float*>(ws);
   }
-  P.vec = sk_vec(q, qs_b, qs_h, qs_t, head_dim, dtype) && sk_vec(k, ks_b, ks_h, ks_t, head_dim, dtype) &&
-          sk_vec(v, vs_b, vs_h, vs_t, head_dim, dtype) && sk_vec(dout, ds_b, ds_h, ds_t, head_dim, dtype);
-  auto run_q = [&](auto t, auto w, auto sp) {
-    using T = decltype(t);
-    constexpr int HD = decltype(w)::value, UN = decltype(sp)::value ? 16 : SK_T;
-    const dim3 grid(static_cast<unsigned>((Tq + UN - 1) / UN * Hq), static_cast<unsigned>(B));
-    sk_launch(&sk_dq_kernel<T, HD, decltype(sp)::value>, grid, sizeof(float) * 2 * SK_T * (HD + 4), st, P);
-  };
-  auto run_kv = [&](auto t, auto w, auto sp) {
-    using T = decltype(t);
-    constexpr int HD = decltype(w)::value, UN = decltype(sp)::value ? 16 : SK_T;
-    SkSinkSplit SU = S;
-    if (S.parts) SU.tiles = (P.sinks + UN - 1) / UN;
-    const dim3 grid(static_cast<unsigned>(((Tk + UN - 1) / UN + SU.tiles * SU.parts) * Hkv), static_cast<unsigned>(B));
-    sk_launch(&sk_dkv_kernel<T, HD, decltype(sp)::value>, grid, sizeof(float) * (2 * SK_T * (HD + 4) + 2 * SK_T), st, P,
-              SU);
-  };
-  sk_by_width(head_dim, [&](auto w) {
-    if (Tq > 0)
-      sk_by_form(dtype, sk_split_waves(Tq, B * Hq), [&](auto t, auto sp) { run_q(t, w, sp); });
-    sk_by_form(dtype, sk_split_waves(Tk, B * Hkv), [&](auto t, auto sp) { run_kv(t, w, sp); });
-  });
-  sum_sinks();
+  if (bf16) {
+    sb_backward(P, S, st);
+  } else {
+    P.vec = sk_vec(q, qs_b, qs_h, qs_t, head_dim, dtype) && sk_vec(k, ks_b, ks_h, ks_t, head_dim, dtype) &&
+            sk_vec(v, vs_b, vs_h, vs_t, head_dim, dtype) && sk_vec(dout, ds_b, ds_h, ds_t, head_dim, dtype);
+    auto run_q = [&](auto t, auto w, auto sp) {
+      using T = decltype(t);
+      constexpr int HD = decltype(w)::value, UN = decltype(sp)::value ? 16 : SK_T;
+      const dim3 grid(static_cast<unsigned>((Tq + UN - 1) / UN * Hq), static_cast<unsigned>(B), P.ksplit);
+      sk_launch(&sk_dq_kernel<T, HD, decltype(sp)::value>, grid, sizeof(float) * 2 * SK_T * (HD + 4), st, P);
+    };
+    auto run_kv = [&](auto t, auto w, auto sp) {
+      using T = decltype(t);
+      constexpr int HD = decltype(w)::value, UN = decltype(sp)::value ? 16 : SK_T;
+      SkSinkSplit SU = S;
+      if (S.parts) SU.tiles = (P.sinks + UN - 1) / UN;
+      const dim3 grid(static_cast<unsigned>(((Tk + UN - 1) / UN + SU.tiles * SU.parts) * Hkv), static_cast<unsigned>(B),
+                      P.hsplit);
+      sk_launch(&sk_dkv_kernel<T, HD, decltype(sp)::value>, grid, sizeof(float) * (2 * SK_T * (HD + 4) + 2 * SK_T), st,
+                P, SU);
+    };
+    sk_by_width(head_dim, [&](auto w) {
+      if (Tq > 0) sk_by_form(dtype, sk_split_waves(Tq, B * Hq), [&](auto t, auto sp) { run_q(t, w, sp); });
+      sk_by_form(dtype, sk_split_waves(Tk, B * Hkv), [&](auto t, auto sp) { run_kv(t, w, sp); });
+    });
+  }
+  sk_join<false>(P, dtype, st);
+  const int rows = P.hsplit > 1 ? P.Tk : (S.parts ? P.sinks : 0);
+  if (rows > 0) {
+    const unsigned blocks = static_cast<unsigned>(B * Hkv * rows);
+    if (dtype == FSI_DTYPE_F32) sk_kv_sum_kernel<float><<<blocks, SK_THREADS, 0, st>>>(P, S, rows);
+    else sk_kv_sum_kernel<bf16_t><<<blocks, SK_THREADS, 0, st>>>(P, S, rows);
+  }
   FSI_HIP_LAUNCH_CHECK("sink_attn_bwd");
   return FSI_OK;
 }

@@ -72,14 +72,14 @@ __global__ __launch_bounds__(SB_THREADS, 2) void sb_fwd_kernel(SkParams P) {
   const bf16_t* k = static_cast<const bf16_t*>(P.k) + b * P.ks_b + g * P.ks_h;
   const bf16_t* v = static_cast<const bf16_t*>(P.v) + b * P.vs_b + g * P.vs_h;
   const SkTiles tiles = sk_key_tiles(P, off + i0, min(off + min(i0 + QW, P.Tq), len) - 1);
-  const int n = tiles.count();
+  const SkRange range = sk_key_part(P, tiles.count(), blockIdx.z);
   auto load = [&](int c) {
-    if (c >= n) return;
+    if (c >= range.hi) return;
     char* dst = smem + (c & 1) * (2 * TB);
     sab_dma<HD, SB_THREADS>(k, P.ks_t, tiles.tile(c) * SK_T, len, dst);
     sab_dma<HD, SB_THREADS>(v, P.vs_t, tiles.tile(c) * SK_T, len, dst + TB);
   };
-  load(0);
+  load(range.lo);
   u32x4_t q[2][KS];
   int hi[2];  // last visible key of query iw + 16 i + r
 #pragma unroll
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(SB_THREADS, 2) void sb_fwd_kernel(SkParams P) {
   };
 
   __syncthreads();  // the first tile is there
-  for (int c = 0; c < n; ++c) {
+  for (int c = range.lo; c < range.hi; ++c) {
     load(c + 1);
     step(c);
     __syncthreads();
@@ -199,6 +199,13 @@ __global__ __launch_bounds__(SB_THREADS, 2) void sb_fwd_kernel(SkParams P) {
   for (int i = 0; i < 2; ++i) {
     const int qi = iw + 16 * i + r;
     if (qi >= P.Tq) continue;
+    if (P.ksplit > 1) {
+      float* row = sk_part_row(P, blockIdx.z, b, h, qi);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t*>(row + 16 * dt + 4 * kg) = acc[i][dt];
+      if (kg == 0) *reinterpret_cast<f32x4_t*>(row + HD) = f32x4_t{m[i], lsum[i][0], l_full[i], 0.f};
+      continue;
+    }
     const float l = lsum[i][0], inv = l == 0.f ? 0.f : 1.f / l;
     bf16_t* o = static_cast<bf16_t*>(P.o) + b * P.os_b + h * P.os_h + qi * P.os_t + 4 * kg;
 #pragma unroll
@@ -230,14 +237,14 @@ __global__ __launch_bounds__(SB_THREADS, 2) void sb_dq_kernel(SkParams P) {
   const bf16_t* k = static_cast<const bf16_t*>(P.k) + b * P.ks_b + g * P.ks_h;
   const bf16_t* v = static_cast<const bf16_t*>(P.v) + b * P.vs_b + g * P.vs_h;
   const SkTiles tiles = sk_key_tiles(P, off + i0, min(off + min(i0 + QW, P.Tq), len) - 1);
-  const int n = tiles.count();
+  const SkRange range = sk_key_part(P, tiles.count(), blockIdx.z);
   auto load = [&](int c) {
-    if (c >= n) return;
+    if (c >= range.hi) return;
     char* dst = smem + (c & 1) * (2 * TB);
     sab_dma<HD, SB_THREADS>(k, P.ks_t, tiles.tile(c) * SK_T, len, dst);
     sab_dma<HD, SB_THREADS>(v, P.vs_t, tiles.tile(c) * SK_T, len, dst + TB);
   };
-  load(0);
+  load(range.lo);
   u32x4_t q[2][KS], gr[2][KS];
   float lse[2], dd[2];
   int hi[2];
@@ -262,7 +269,7 @@ __global__ __launch_bounds__(SB_THREADS, 2) void sb_dq_kernel(SkParams P) {
     dd[i] = sum_rows4(d);
     lse[i] = live ? P.lse[stat + qi] : INFINITY;
     hi[i] = live ? off + qi : -1;
-    if (qi < P.Tq && kg == 0) P.dd[stat + qi] = dd[i];
+    if (qi < P.Tq && kg == 0 && blockIdx.z == 0) P.dd[stat + qi] = dd[i];
   }
   const float sl2 = P.scale * SB_LOG2E;
   f32x4_t acc[2][DT];
@@ -272,7 +279,7 @@ __global__ __launch_bounds__(SB_THREADS, 2) void sb_dq_kernel(SkParams P) {
     for (int dt = 0; dt < DT; ++dt) acc[i][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   const uint32_t row_off = sab_row_off<HD>(r, kg), tr_off = sab_tr_off<HD>(r, kg);
   __syncthreads();
-  for (int c = 0; c < n; ++c) {
+  for (int c = range.lo; c < range.hi; ++c) {
     load(c + 1);
     const int s0 = tiles.tile(c) * SK_T;
 #pragma unroll 1
@@ -335,6 +342,12 @@ __global__ __launch_bounds__(SB_THREADS, 2) void sb_dq_kernel(SkParams P) {
   for (int i = 0; i < 2; ++i) {
     const int qi = iw + 16 * i + r;
     if (qi >= P.Tq) continue;
+    if (P.ksplit > 1) {
+      float* row = sk_part_row(P, blockIdx.z, b, h, qi);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t*>(row + 16 * dt + 4 * kg) = acc[i][dt] * P.scale;
+      continue;
+    }
     bf16_t* o = static_cast<bf16_t*>(P.dq) + (stat + qi) * HD + 4 * kg;
     const float f = P.scale;
 #pragma unroll
@@ -394,14 +407,15 @@ __global__ __launch_bounds__(SB_THREADS, 2) void sb_dkv_kernel(SkParams P, SkSin
       __builtin_amdgcn_global_load_lds((ab_glb_t*)st, (ab_lds_t*)(dst + 2 * TB + wave * AB_T * 4), 4, 0, 0);
     }
   };
-  int i = i_lo, hh = 0, stage = 0;
+  const SkRange heads = sk_head_part(P, blockIdx.z);
+  int i = heads.lo < heads.hi ? i_lo : i_hi, hh = heads.lo, stage = 0;
   if (i < i_hi) load(i, hh, 0);
   __syncthreads();
   while (i < i_hi) {
     const int t0 = i, cur = stage * STAGE;
     stage ^= 1;
-    if (++hh == G) {
-      hh = 0;
+    if (++hh == heads.hi) {
+      hh = heads.lo;
       i += SK_T;
     }
     if (i < i_hi) load(i, hh, stage);
@@ -496,10 +510,10 @@ __global__ __launch_bounds__(SB_THREADS, 2) void sb_dkv_kernel(SkParams P, SkSin
     for (int dt = 0; dt < DT; ++dt) {
       const f32x4_t ka = (dka[kt][dt] + sums[(2 * (kt * DT + dt)) * 64]) * P.scale;
       const f32x4_t va = dva[kt][dt] + sums[(2 * (kt * DT + dt) + 1) * 64];
-      if (n_far > 0 && s < P.sinks) {  // a term of the row's sum: the window's is the last one
-        float* t = S.sums + (((head * (S.parts + 1) + (part < 0 ? S.parts : part)) * P.sinks + s) * 2) * HD + 16 * dt + 4 * kg;
-        *reinterpret_cast<f32x4_t*>(t) = ka;
-        *reinterpret_cast<f32x4_t*>(t + HD) = va;
+      if (float* t = sk_kv_term(P, S, head, s, blockIdx.z, part)) {
+        if (part >= 0 && s >= P.sinks) continue;
+        *reinterpret_cast<f32x4_t*>(t + 16 * dt + 4 * kg) = ka;
+        *reinterpret_cast<f32x4_t*>(t + HD + 16 * dt + 4 * kg) = va;
       } else if (part < 0) {
         const int64_t at = (head * P.Tk + s) * HD + 16 * dt + 4 * kg;
         *reinterpret_cast<u32x2_t*>(static_cast<bf16_t*>(P.dk) + at) = u32x2_t{bf_cvt2(ka[0], ka[1]), bf_cvt2(ka[2], ka[3])};
@@ -534,12 +548,18 @@ static int sb_heads(const SkParams& P, int most) {
   return 1;
 }
 
+int64_t sb_query_blocks(const SkParams& P, bool backward) {
+  const int64_t heads = sb_heads(P, backward ? 2 : 4), queries = SB_WAVES / heads * 32;
+  return (P.Tq + queries - 1) / queries * (P.Hq / heads) * P.B;
+}
+
 void sb_forward(const SkParams& P, hipStream_t st) {
   auto run = [&](auto hd) {
     constexpr int HD = decltype(hd)::value;
     auto launch = [&](auto heads) {
       constexpr int HPW = decltype(heads)::value, QW = SB_WAVES / HPW * 32;
-      const dim3 grid(static_cast<unsigned>((P.Tq + QW - 1) / QW * (P.Hq / HPW)), static_cast<unsigned>(P.B));
+      const dim3 grid(static_cast<unsigned>((P.Tq + QW - 1) / QW * (P.Hq / HPW)), static_cast<unsigned>(P.B),
+                      P.ksplit);
       if (P.lse) sb_fwd_kernel<HD, HPW, true><<<grid, SB_THREADS, 0, st>>>(P);
       else sb_fwd_kernel<HD, HPW, false><<<grid, SB_THREADS, 0, st>>>(P);
     };
@@ -558,13 +578,15 @@ void sb_backward(const SkParams& P, const SkSinkSplit& S, hipStream_t st) {
     constexpr int HD = decltype(hd)::value;
     auto launch = [&](auto heads) {
       constexpr int HPW = decltype(heads)::value, QW = SB_WAVES / HPW * 32;
-      const dim3 grid(static_cast<unsigned>((P.Tq + QW - 1) / QW * (P.Hq / HPW)), static_cast<unsigned>(P.B));
+      const dim3 grid(static_cast<unsigned>((P.Tq + QW - 1) / QW * (P.Hq / HPW)), static_cast<unsigned>(P.B),
+                      P.ksplit);
       sb_dq_kernel<HD, HPW><<<grid, SB_THREADS, 0, st>>>(P);
     };
     if (sb_heads(P, 2) == 2) launch(std::integral_constant<int, 2>{});
     else launch(std::integral_constant<int, 1>{});
     const unsigned tiles = static_cast<unsigned>((P.Tk + SK_T - 1) / SK_T + S.tiles * S.parts);
-    sb_dkv_kernel<HD><<<dim3(tiles * static_cast<unsigned>(P.Hkv), static_cast<unsigned>(P.B)), SB_THREADS, 0, st>>>(P, S);
+    sb_dkv_kernel<HD><<<dim3(tiles * static_cast<unsigned>(P.Hkv), static_cast<unsigned>(P.B), P.hsplit), SB_THREADS, 0,
+                        st>>>(P, S);
   };
   if (P.hd == 128) run(std::integral_constant<int, 128>{});
   else run(std::integral_constant<int, 64>{});

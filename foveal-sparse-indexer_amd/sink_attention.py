@@ -46,11 +46,15 @@ def _fwd_op(q: Tensor, k: Tensor, v: Tensor, lengths: Optional[Tensor], window: 
     B, Hq, Tq, hd = q.shape
     out = _out_like(q)
     lse = torch.empty((B, Hq, Tq) if want_lse else (0,), dtype=torch.float32, device=dev)
+    L = _lib.lib()
+    Hkv, Tk = k.shape[1], k.shape[2]
+    need = L.fsi_sink_attn_workspace_size(B, Hq, Hkv, Tq, Tk, hd, window, sinks)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     with _lib.device_guard(dev):
-        st = _lib.lib().fsi_sink_attn(
-            q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], B, Hq,
-            k.shape[1], Tq, k.shape[2], hd, window, sinks, _lib.ptr(lengths), scale, _lib.dtype_code(q.dtype, _WHAT),
-            out.data_ptr(), *out.stride()[:3], lse.data_ptr() if want_lse else None, _lib.stream_handle(dev))
+        st = L.fsi_sink_attn(
+            q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], B, Hq, Hkv,
+            Tq, Tk, hd, window, sinks, _lib.ptr(lengths), scale, _lib.dtype_code(q.dtype, _WHAT), out.data_ptr(),
+            *out.stride()[:3], lse.data_ptr() if want_lse else None, _lib.ptr(ws), need, _lib.stream_handle(dev))
     _lib.check(st, _WHAT)
     return out, lse
 

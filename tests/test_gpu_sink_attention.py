@@ -98,6 +98,31 @@ def test_sinks_seen_from_afar(fsi, dev, dtype, hd, Hq, Hkv, Tq, Tk, window, sink
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("hd", [64, 128, 48])
+@pytest.mark.parametrize("Hq,Hkv,Tq,Tk,window,sinks,lengths", [
+    (4, 1, 1, 2100, 2100, 0, None),  # one query, all keys
+    (2, 1, 20, 1500, 1400, 70, [1490]),  # sinks and a long window
+    (8, 1, 300, 300, 300, 3, None),  # one KV head for all
+    (6, 2, 130, 1030, 1000, 4, [900]),  # no query inside the length
+])
+def test_few_rows_over_many_keys(fsi, dev, dtype, hd, Hq, Hkv, Tq, Tk, window, sinks, lengths):
+    """Keys (query heads) cut into parts that are joined at the end."""
+    q, k, v, dout = _inputs(1, Hq, Hkv, Tq, Tk, hd, dtype, seed=Tk)
+    n = None if lengths is None else torch.tensor(lengths)
+    got = _run(fsi, dev, q, k, v, dout, window=window, sinks=sinks, lengths=None if n is None else n.to(dev))
+    _check(got, *oracle.attention(q, k, v, dout, window, sinks, n, 1 / math.sqrt(hd), *UNIT[dtype]))
+
+
+@pytest.mark.parametrize("dtype,hd", [(BF16, 64), (BF16, 128), (BF16, 40), (F32, 64)])
+def test_more_tiles_than_compute_units(fsi, dev, dtype, hd):
+    """Enough heads for a workgroup on every compute unit: nothing but the sinks is cut."""
+    q, k, v, dout = _inputs(2, 18, 9, 1000, 1000, hd, dtype, seed=hd)
+    lengths = torch.tensor([1000, 950])
+    got = _run(fsi, dev, q, k, v, dout, window=100, sinks=4, lengths=lengths.to(dev))
+    _check(got, *oracle.attention(q, k, v, dout, 100, 4, lengths, 1 / math.sqrt(hd), *UNIT[dtype]))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_memory_behind_the_lengths_is_not_used(fsi, dev, dtype):
     q, k, v, dout = _inputs(2, 2, 1, 150, 150, 64, dtype, seed=3)
     lengths = torch.tensor([100, 1])

@@ -78,7 +78,7 @@ def test_sink_attention_errors(fsi):
 
     def fwd(q=_ptr(1), B=1, Hq=4, Hkv=2, Tq=3, Tk=5, hd=64, window=2, sinks=1, dtype=1):
         return L.fsi_sink_attn(q, 1, 1, 1, _ptr(2), 1, 1, 1, _ptr(3), 1, 1, 1, B, Hq, Hkv, Tq, Tk, hd, window, sinks,
-                               None, 1.0, dtype, _ptr(4), 1, 1, 1, None, None)
+                               None, 1.0, dtype, _ptr(4), 1, 1, 1, None, None, 0, None)
 
     def bwd(q=_ptr(1), Tq=3, Tk=5, hd=64, dtype=1, ws=None, nbytes=0, dk=_ptr(8)):
         return L.fsi_sink_attn_bwd(q, 1, 1, 1, _ptr(2), 1, 1, 1, _ptr(3), 1, 1, 1, _ptr(4), 1, 1, 1, _ptr(5), 1, 1, 1,
@@ -90,6 +90,8 @@ def test_sink_attention_errors(fsi):
     assert fwd(window=-1) == _lib.FSI_ERR_SHAPE and fwd(sinks=-1) == _lib.FSI_ERR_SHAPE
     assert fwd(Tk=1 << 31) == _lib.FSI_ERR_SHAPE and fwd(q=None) == _lib.FSI_ERR_INVALID_ARG
     assert fwd(Tq=0, q=None) == _lib.FSI_OK and fwd(B=0, q=None) == _lib.FSI_OK
+    assert fwd(Tq=1, Tk=8192, window=8192) == _lib.FSI_ERR_WORKSPACE  # one query over many keys runs in parts
+    assert L.fsi_sink_attn_workspace_size(1, 4, 2, 1, 8192, 64, 8192, 0) > 0
     assert bwd(dtype=3) == _lib.FSI_ERR_DTYPE and bwd(hd=300) == _lib.FSI_ERR_SHAPE
     assert bwd(q=None) == _lib.FSI_ERR_INVALID_ARG and bwd(dk=None) == _lib.FSI_ERR_INVALID_ARG
     assert bwd() == _lib.FSI_ERR_WORKSPACE
