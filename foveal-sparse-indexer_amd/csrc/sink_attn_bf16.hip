@@ -1,4 +1,4 @@
-// Windowed attention with sinks (sink_attn.h) for bf16 with head_dim 64 or 128: forward, dQ, and
+// Windowed attention with sinks (sink_attn.h) for bf16 with head_dim 64, 128 or 256: forward, dQ, and
 // dK / dV, every product on v_mfma_f32_16x16x32_bf16 over 64-row LDS tiles (attn_tiles_bf16.h)
 // that direct-to-LDS loads fill one step ahead.
 //
@@ -53,9 +53,11 @@ __device__ __forceinline__ SbKeys sb_keys(const SkParams& P, int len, int a, int
 // ---------------------------------------------------------------------------
 constexpr int SB_THREADS = 256;
 constexpr int SB_WAVES = SB_THREADS / 64;
+// Workgroups a CU that a kernel's registers and LDS are kept to: head_dim 256 takes all of one.
+constexpr int sb_blocks(int hd) { return hd > 128 ? 1 : 2; }
 
 template <int HD, int HPW, bool LSE>
-__global__ __launch_bounds__(SB_THREADS, 2) void sb_fwd_kernel(SkParams P) {
+__global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_fwd_kernel(SkParams P) {
   constexpr int KS = HD / 32, DT = HD / 16, TB = sab_tile_bytes<HD>();
   constexpr int QW = SB_WAVES / HPW * 32;  // queries of a workgroup
   __shared__ __attribute__((aligned(1024))) char smem[2 * 2 * TB];  // [stage][K, V]
@@ -222,7 +224,7 @@ __global__ __launch_bounds__(SB_THREADS, 2) void sb_fwd_kernel(SkParams P) {
 // 64 * 2 / HPW queries; a wave is one head's 32 queries over 32 keys at a time.
 // ---------------------------------------------------------------------------
 template <int HD, int HPW>
-__global__ __launch_bounds__(SB_THREADS, 2) void sb_dq_kernel(SkParams P) {
+__global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_dq_kernel(SkParams P) {
   constexpr int KS = HD / 32, DT = HD / 16, TB = sab_tile_bytes<HD>();
   constexpr int QW = SB_WAVES / HPW * 32;
   __shared__ __attribute__((aligned(1024))) char smem[2 * 2 * TB];  // [stage][K, V]
@@ -363,7 +365,7 @@ __global__ __launch_bounds__(SB_THREADS, 2) void sb_dq_kernel(SkParams P) {
 // The first S.tiles * S.parts workgroups of a KV head are the split sink tiles' (SkSinkSplit).
 // ---------------------------------------------------------------------------
 template <int HD>
-__global__ __launch_bounds__(SB_THREADS, 2) void sb_dkv_kernel(SkParams P, SkSinkSplit S) {
+__global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_dkv_kernel(SkParams P, SkSinkSplit S) {
   constexpr int KS = HD / 32, DT = HD / 16, TB = sab_tile_bytes<HD>();
   constexpr int STAGE = 2 * TB + 2 * AB_T * 4;    // Q, dout, then lse and D of the rows
   constexpr int SUMS = 2 * 2 * 2 * DT * 64 * 16;  // two waves' dK and dV accumulators
@@ -532,7 +534,7 @@ bool sb_takes(const SkParams& P, int dtype, bool backward) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && sb % 8 == 0 && sh % 8 == 0 && st % 8 == 0 && st >= 0 &&
            st < (int64_t(1) << 24);
   };
-  return dtype == FSI_DTYPE_BF16 && (P.hd == 64 || P.hd == 128) && P.scale > 0.f && P.Tq > 0 &&
+  return dtype == FSI_DTYPE_BF16 && (P.hd == 64 || P.hd == 128 || P.hd == 256) && P.scale > 0.f && P.Tq > 0 &&
          rows(P.q, P.qs_b, P.qs_h, P.qs_t) && rows(P.k, P.ks_b, P.ks_h, P.ks_t) && rows(P.v, P.vs_b, P.vs_h, P.vs_t) &&
          rows(P.o, P.os_b, P.os_h, P.os_t) &&
          (!backward || (rows(P.dout, P.ds_b, P.ds_h, P.ds_t) &&
@@ -569,7 +571,8 @@ void sb_forward(const SkParams& P, hipStream_t st) {
       default: launch(std::integral_constant<int, 1>{});
     }
   };
-  if (P.hd == 128) run(std::integral_constant<int, 128>{});
+  if (P.hd == 256) run(std::integral_constant<int, 256>{});
+  else if (P.hd == 128) run(std::integral_constant<int, 128>{});
   else run(std::integral_constant<int, 64>{});
 }
 
@@ -588,7 +591,8 @@ void sb_backward(const SkParams& P, const SkSinkSplit& S, hipStream_t st) {
     sb_dkv_kernel<HD><<<dim3(tiles * static_cast<unsigned>(P.Hkv), static_cast<unsigned>(P.B), P.hsplit), SB_THREADS, 0,
                         st>>>(P, S);
   };
-  if (P.hd == 128) run(std::integral_constant<int, 128>{});
+  if (P.hd == 256) run(std::integral_constant<int, 256>{});
+  else if (P.hd == 128) run(std::integral_constant<int, 128>{});
   else run(std::integral_constant<int, 64>{});
 }
 

@@ -10,11 +10,26 @@ import math
 from typing import Optional, Tuple
 
 import torch
+import torch.nn.functional as F
 from torch import Tensor
 
 from . import _lib
 
 _WHAT = "sink_window_attention"
+_MFMA_WIDTHS = (64, 128, 256)  # head_dims of the bf16 MFMA kernels
+# Products (queries x keys x head_dim) from which bf16 heads of other sizes are padded with zeros to
+# the next of them: the copies cost 30-40 us of host time, 90 with gradients.  8 heads of 96 over
+# 1024 tokens, window 512 (4e8): 291 us with gradients on fp32 MFMA, 275 padded; 40 (2e8): 203 and
+# 269; 200 (8e8): 849 and 283; 2 x 4096 tokens, 32 heads of 96: 5247 and 811.
+_PAD_WORK = 1 << 29
+
+
+def _width(q: Tensor, keys: int) -> int:
+    """head_dim to run q at."""
+    hd = q.shape[3]
+    if q.dtype != torch.bfloat16 or hd in _MFMA_WIDTHS or q.numel() * keys < _PAD_WORK:
+        return hd
+    return next((w for w in _MFMA_WIDTHS if w > hd), hd)
 
 
 def _rows(t: Tensor) -> Tensor:
@@ -22,7 +37,7 @@ def _rows(t: Tensor) -> Tensor:
     the bf16 MFMA kernels cannot read in 16-byte pieces are copied."""
     if t.stride(3) != 1:
         return t.contiguous()
-    if (t.dtype == torch.bfloat16 and t.shape[3] in (64, 128)
+    if (t.dtype == torch.bfloat16 and t.shape[3] in _MFMA_WIDTHS
             and (t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:3]))):
         return t.clone(memory_format=torch.contiguous_format)
     return t
@@ -125,7 +140,7 @@ def sink_window_attention(
     Inside a length, v where it is hidden enters as 0 times the value, in the gradients q, k
     and the incoming gradient as well, so they have to be finite; hidden k may hold anything
     in the forward.  Returns (B, Hq, Tq, hd), a view of a
-    (B, Tq, Hq, hd) buffer."""
+    (B, Tq, Hq, hd) buffer (of padded heads where hd is not a size of the MFMA kernels)."""
     dev = _lib.require_gpu(q, k, v, lengths, what=_WHAT)
     if not (q.dtype == k.dtype == v.dtype):
         raise TypeError(f"{_WHAT}: q, k, v dtypes {q.dtype}, {k.dtype}, {v.dtype} differ")
@@ -146,6 +161,14 @@ def sink_window_attention(
             raise ValueError(f"{_WHAT}: lengths must be {B} integers, got {tuple(lengths.shape)} {lengths.dtype}")
         lengths = lengths.to(device=dev, dtype=torch.int32).reshape(-1).contiguous()
     args = (lengths, int(window), int(sinks), float(scale))
+    width = _width(q, min(Tk, window + sinks))
+    if width != hd:
+        q, k, v = (F.pad(t, (0, width - hd)) for t in (q, k, v))
+        return _attend(q, k, v, args)[..., :hd]
+    return _attend(q, k, v, args)
+
+
+def _attend(q: Tensor, k: Tensor, v: Tensor, args) -> Tensor:
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _SinkAttnFn.apply(_rows(q), _rows(k), _rows(v), *args)
     return _fwd_op(_rows(q.detach()), _rows(k.detach()), _rows(v.detach()), *args, False)[0]

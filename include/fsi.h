@@ -655,7 +655,7 @@ FSI_API int fsi_sparse_attn_bwd(const void* q, int64_t qs_b, int64_t qs_h, int64
  * sees no key gets 0; the memory behind a sequence's length is not used.  Query head h
  * uses KV head h / (Hq / Hkv).  Element strides over (B, H, T), unit stride over
  * head_dim 1..256; dtype FSI_DTYPE_BF16 or FSI_DTYPE_F32, fp32 softmax and sums.  bf16 with
- * head_dim 64 or 128, 16-byte aligned pointers and strides of multiples of 8 elements
+ * head_dim 64, 128 or 256, 16-byte aligned pointers and strides of multiples of 8 elements
  * runs on bf16 MFMA, everything else on fp32 MFMA.
  * lse (B, Hq, Tq) fp32 (null: not wanted): log2 of each query's softmax denominator in
  * units of scale log2(e) q.k, which the backward takes; +inf for a query without keys.

@@ -74,6 +74,17 @@ def test_head_sizes(fsi, dev, dtype, hd):
     _check(got, *oracle.attention(q, k, v, dout, 30, 2, None, 0.3, *UNIT[dtype]))
 
 
+@pytest.mark.parametrize("hd", [20, 96, 200, 256])
+def test_padded_heads(fsi, dev, hd, monkeypatch):
+    """bf16 heads of other sizes, padded to the MFMA kernels' next size as large calls are."""
+    from foveal_sparse_indexer_amd import sink_attention
+
+    monkeypatch.setattr(sink_attention, "_PAD_WORK", 0)
+    q, k, v, dout = _inputs(1, 8, 4, 600, 600, hd, BF16, seed=hd)
+    got = _run(fsi, dev, q, k, v, dout, window=300, sinks=4)
+    _check(got, *oracle.attention(q, k, v, dout, 300, 4, None, 1 / math.sqrt(hd), *UNIT[BF16]))
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("hd", [64, 128])
 def test_longer_rows(fsi, dev, dtype, hd):
