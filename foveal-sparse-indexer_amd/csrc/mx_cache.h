@@ -80,60 +80,7 @@ __device__ __forceinline__ int mx_scale_byte(uint32_t amax) {
   return e + 127;
 }
 
-// 2^(byte - 127) and its inverse, exact for bytes of finite groups.
+// 2^(byte - 127), exact for bytes of finite groups.
 __device__ __forceinline__ float mx_scale(int byte) { return __uint_as_float(static_cast<uint32_t>(byte) << 23); }
-__device__ __forceinline__ float mx_inv_scale(int byte) {
-  return __uint_as_float(static_cast<uint32_t>(254 - byte) << 23);
-}
-
-// Element code of y = x 2^-e: |y| rounded to the spacing of its binade (spacing of the lowest
-// binade below it), clamped, sign in the top bit.  fp4: spacing 0.5 below 2, 1 below 4, else 2;
-// the code of value v is the index in the value list: 2 v below 2, v + 2 below 4, v / 2 + 4.
-__device__ __forceinline__ uint32_t mx_fp4_code(float y) {
-  const uint32_t sign = __float_as_uint(y) >> 31;
-  const float a = fminf(fabsf(y), 6.f);
-  const float step = a < 2.f ? 2.f : (a < 4.f ? 1.f : 0.5f);
-  const int n = static_cast<int>(rintf(a * step));  // steps of the binade's spacing
-  const int code = a < 2.f ? n : (a < 4.f ? n + 2 : n + 4);
-  return static_cast<uint32_t>(code) | (sign << 3);
-}
-// e4m3: |y| below 2^-6 has spacing 2^-9.  The fp32 bit pattern rounded at the 3-bit mantissa
-// (a carry moves into the exponent by itself), then rebiased.
-__device__ __forceinline__ uint32_t mx_fp8_code(float y) {
-  const uint32_t sign = (__float_as_uint(y) >> 31) << 7;
-  const float a = fminf(fabsf(y), 448.f);
-  uint32_t code;
-  if (a < 0.015625f) {
-    code = static_cast<uint32_t>(rintf(a * 512.f));  // 8 = the smallest normal number's code
-  } else {
-    uint32_t u = __float_as_uint(a);
-    u += 0x7ffffu + ((u >> 20) & 1u);
-    code = (u >> 20) - ((127 - 7) << 3);
-  }
-  return code | sign;
-}
-template <int FMT>
-__device__ __forceinline__ uint32_t mx_code(float y) {
-  return FMT == FMT_FP4 ? mx_fp4_code(y) : mx_fp8_code(y);
-}
-
-// Value of an element code, without its scale.
-__device__ __forceinline__ float mx_fp4_value(uint32_t c) {
-  const uint32_t m = c & 7u;
-  const float a = m < 4 ? 0.5f * m : (m < 6 ? static_cast<float>(m) - 2.f : 2.f * m - 8.f);
-  return c & 8u ? -a : a;
-}
-__device__ __forceinline__ float mx_fp8_value(uint32_t c) {
-  const uint32_t m = c & 0x7fu;
-  float a;
-  if (m == 0x7fu) a = __uint_as_float(0x7fc00000u);
-  else if (m < 8) a = m * 0.001953125f;
-  else a = __uint_as_float((m << 20) + ((127u - 7u) << 23));
-  return c & 0x80u ? -a : a;
-}
-template <int FMT>
-__device__ __forceinline__ float mx_value(uint32_t c) {
-  return FMT == FMT_FP4 ? mx_fp4_value(c) : mx_fp8_value(c);
-}
 
 }  // namespace fsi_mx
