@@ -432,6 +432,8 @@ def _decode_sinks_launch(q3: Tensor, k_cache: Tensor, v_cache: Tensor, fmt: int,
     workspace, so graphs captured on one stream may be replayed side by side."""
     what = "decode_attention"
     dev = q3.device
+    if q3.data_ptr() % 16:  # a view: the kernels read 16-byte pieces
+        q3 = q3.clone()
     B, Hq, hd = q3.shape
     L = _lib.lib()
     err = _lib.error_word(dev)
@@ -609,8 +611,6 @@ def _decode_attention_sinks(q3: Tensor, cache: FovealKVCache, pos_rows: Optional
         raise ValueError(f"{what}: pages {tuple(remote_pages.shape)} / counts {tuple(remote_counts.shape)} are not "
                          f"(B, capacity) / (B,) for {B} sequences")
     q3 = q3.detach().contiguous()
-    if q3.data_ptr() % 16:
-        q3 = q3.clone()
     args = (cache.k_cache, cache.v_cache, _lib.KV_FORMATS[cache.kv_format], cache.page_table, cache.max_pages,
             cache.n_phys_pages, cache.num_kv_heads, pos_rows, pos_val, window, sinks, remote_pages, remote_counts,
             cap, scale)

@@ -58,6 +58,7 @@ def _fwd_op(q: Tensor, k: Tensor, v: Tensor, lengths: Optional[Tensor], window: 
             want_lse: bool) -> Tuple[Tensor, Tensor]:
     """fsi_sink_attn: (out (B, Hq, Tq, hd), lse (B, Hq, Tq) or empty)."""
     dev = q.device
+    q, k, v = _rows(q), _rows(k), _rows(v)
     B, Hq, Tq, hd = q.shape
     out = _out_like(q)
     lse = torch.empty((B, Hq, Tq) if want_lse else (0,), dtype=torch.float32, device=dev)
@@ -83,6 +84,7 @@ def _bwd_op(q: Tensor, k: Tensor, v: Tensor, out: Tensor, dout: Tensor, lse: Ten
             window: int, sinks: int, scale: float) -> Tuple[Tensor, Tensor, Tensor]:
     """fsi_sink_attn_bwd: contiguous (dq, dk, dv) of the operands' dtype."""
     dev = q.device
+    q, k, v, out, dout = (_rows(t) for t in (q, k, v, out, dout))
     B, Hq, Tq, hd = q.shape
     Hkv, Tk = k.shape[1], k.shape[2]
     dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
@@ -114,7 +116,7 @@ class _SinkAttnFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, lengths = ctx.saved_tensors
-        grads = _bwd_op(q, k, v, out, _rows(dout.to(q.dtype)), lse, lengths, *ctx.meta)
+        grads = _bwd_op(q, k, v, out, dout.to(q.dtype), lse, lengths, *ctx.meta)
         return (*grads, None, None, None, None)
 
 
@@ -170,5 +172,5 @@ def sink_window_attention(
 
 def _attend(q: Tensor, k: Tensor, v: Tensor, args) -> Tensor:
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _SinkAttnFn.apply(_rows(q), _rows(k), _rows(v), *args)
-    return _fwd_op(_rows(q.detach()), _rows(k.detach()), _rows(v.detach()), *args, False)[0]
+        return _SinkAttnFn.apply(q, k, v, *args)
+    return _fwd_op(q.detach(), k.detach(), v.detach(), *args, False)[0]
