@@ -208,6 +208,8 @@ class FovealKVCache:
         self.partial_vp = torch.zeros(batch_size, page_size, index_dim, device=self.device, dtype=dtype)
         self.seq_len = 0
         self.completed_pages = 0
+        if kv_format is not None and self.k_cache.is_cuda:
+            _lib.error_word(self.k_cache.device)  # made here, so that a first write may be captured into a graph
 
     def _write(self, k: Tensor, v: Tensor, start: int | Tensor) -> None:
         what = "FovealKVCache"

@@ -511,7 +511,11 @@ struct MdSplit {
 constexpr int64_t MD_SLOTS = 2048;
 MdSplit md_split(int64_t pairs, int64_t hd, int format, int64_t window, int64_t sinks, int64_t cap,
                  int64_t max_pages) {
-  const int64_t tok = md_tok(format, hd);
+  const int64_t tok = md_tok(format, hd), most_int = 0x7fffffff;
+  window = std::min(window, most_int);
+  sinks = std::min(sinks, most_int);
+  cap = std::min(cap, most_int);
+  max_pages = std::min(max_pages, most_int / MX_PAGE);
   const int64_t all = max_pages * (MX_PAGE / tok);
   const int64_t local = std::min<int64_t>(window / tok + 2, all);
   const int64_t chunks = std::min<int64_t>((sinks + tok - 1) / tok, all) + local + cap * (MX_PAGE / tok);
@@ -534,7 +538,7 @@ FSI_API size_t fsi_decode_attn_sinks_workspace_size(int64_t B, int64_t Hq, int64
                                                     int64_t window, int64_t sinks, int64_t capacity,
                                                     int64_t max_pages) {
   if (B <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || head_dim <= 0 || head_dim > 256 || max_pages <= 0 ||
-      window < 0 || sinks < 0 || capacity < 0 || format < FSI_KV_BF16 || format > FSI_KV_MXFP4)
+      window < 0 || sinks < 0 || capacity < 0 || B > 0x7fffffff / Hkv || format < FSI_KV_BF16 || format > FSI_KV_MXFP4)
     return 0;
   const int64_t pairs = B * Hkv * md_subs(Hq, Hkv);
   const MdSplit s = md_split(pairs, head_dim, format, window, sinks, capacity, max_pages);
@@ -557,6 +561,7 @@ FSI_API int fsi_decode_attn_sinks(const void* q, int dtype, const void* k_pool, 
                 (long long)head_dim);
   FSI_CHECK_ARG(B >= 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0, FSI_ERR_SHAPE,
                 "decode_attn_sinks: B %lld, Hq %lld, Hkv %lld", (long long)B, (long long)Hq, (long long)Hkv);
+  FSI_CHECK_ARG(B <= 0x7fffffff / Hq, FSI_ERR_SHAPE, "decode_attn_sinks: B * Hq beyond int32");
   FSI_CHECK_ARG(max_pages > 0 && n_phys_pages > 0 && window >= 0 && sinks >= 0 && pos >= 0 && capacity >= 0,
                 FSI_ERR_SHAPE, "decode_attn_sinks: bad sizes");
   FSI_CHECK_ARG(max_pages <= 0x7fffffff / MX_PAGE && B <= 0x7fffffff && Hq <= 0x7fffffff && capacity <= 0x1000000,
