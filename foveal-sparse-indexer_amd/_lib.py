@@ -208,12 +208,12 @@ SIGNATURES: dict[str, tuple] = {
     "fsi_sink_attn": (
         _c_int,
         [_c_ptr, _c_i64, _c_i64, _c_i64] * 3 + [_c_i64] * 8 + [_c_ptr, ctypes.c_float, _c_int, _c_ptr, _c_i64, _c_i64,
-                                                             _c_i64, _c_ptr, _c_ptr, _c_size, _c_ptr],
+                                                             _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_size, _c_ptr],
     ),
     "fsi_sink_attn_bwd_workspace_size": (_c_size, [_c_i64] * 8),
     "fsi_sink_attn_bwd": (
         _c_int,
-        [_c_ptr, _c_i64, _c_i64, _c_i64] * 5 + [_c_ptr] + [_c_i64] * 8
+        [_c_ptr, _c_i64, _c_i64, _c_i64] * 4 + [_c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr] + [_c_i64] * 8
         + [_c_ptr, ctypes.c_float, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_size, _c_ptr],
     ),
     "fsi_sram_indexer_attention": (

@@ -23,6 +23,7 @@ struct SkParams {
   int64_t vs_b, vs_h, vs_t;
   void* o;  // forward: written
   int64_t os_b, os_h, os_t;
+  void* olo;  // bf16, laid out as o: what rounding took from it, so that D keeps 16 bits; or null
   const void* dout;
   int64_t ds_b, ds_h, ds_t;
   int B, Hq, Hkv, Tq, Tk, hd, window, sinks;
@@ -112,6 +113,19 @@ __device__ __forceinline__ float* sk_kv_term(const SkParams& P, const SkSinkSpli
 
 __device__ __forceinline__ bool sk_visible(const SkParams& P, int len, int p, int s) {
   return s <= p && (s > p - P.window || s < P.sinks) && p < len;
+}
+
+// The key of a query at position p that sees one key only, else -1.  Its P is 1 and its dS is 0: with
+// D = dout . v, summed as dP is, the kernels' dP - D is 0 to the bit, whatever out was rounded to.
+__device__ __forceinline__ int sk_only_key(const SkParams& P, int p) {
+  if (P.window > 0) return p == 0 || (P.window == 1 && P.sinks == 0) ? p : -1;
+  return P.sinks > 0 && (p == 0 || P.sinks == 1) ? 0 : -1;
+}
+
+// Column r's element (r, r) of a 16 x 16 product, in every lane of the column.
+__device__ __forceinline__ float sk_diagonal(fsi::f32x4_t x, int r, int kg) {
+  const float lo = r & 1 ? x[1] : x[0], hi = r & 1 ? x[3] : x[2];
+  return fsi::sum_rows4(kg == r >> 2 ? (r & 2 ? hi : lo) : 0.f);
 }
 
 // End of the queries that reach key tile s0 before the split's parts begin, in whole query tiles.

@@ -106,6 +106,14 @@ __device__ __forceinline__ void sk_store(T* row, int hd, int kg, const f32x4_t (
       if (16 * dt + 4 * kg + j < hd) sk_st(row + 16 * dt + 4 * kg + j, acc[dt][j] * f);
 }
 
+// One output value, and what rounding took from it where that is kept.
+template <typename T>
+__device__ __forceinline__ void sk_out(const SkParams& P, int64_t at, float x) {
+  sk_st(static_cast<T*>(P.o) + at, x);
+  if constexpr (sizeof(T) == 2)
+    if (P.olo) static_cast<bf16_t*>(P.olo)[at] = f32_to_bf16(x - round_bf16(x));
+}
+
 // SPLIT kernels: the four waves own the same 16 columns and a 16-row part of every tile each, and
 // their sums meet in LDS at the end.  Taken where workgroups of 64 columns would leave CUs without
 // one (rule and figures at sk_split_waves): a quarter of the work behind one another, in four times
@@ -218,7 +226,13 @@ __global__ __launch_bounds__(SK_THREADS) void sk_fwd_kernel(SkParams P) {
     if (kg == 0) *reinterpret_cast<f32x4_t*>(row + sk_part_stride(P.hd) - 4) = f32x4_t{m, l, l, 0.f};
     return;
   }
-  sk_store<T, HD>(static_cast<T*>(P.o) + b * P.os_b + h * P.os_h + i * P.os_t, P.hd, kg, acc, l == 0.f ? 0.f : 1.f / l);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t at = b * P.os_b + h * P.os_h + i * P.os_t;
+#pragma unroll
+  for (int dt = 0; dt < HD / 16; ++dt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (16 * dt + 4 * kg + j < P.hd) sk_out<T>(P, at + 16 * dt + 4 * kg + j, acc[dt][j] * inv);
   if (P.lse && kg == 0)
     P.lse[(static_cast<int64_t>(b) * P.Hq + h) * P.Tq + i] = l == 0.f ? INFINITY : m + __log2f(l);
 }
@@ -241,12 +255,21 @@ __global__ __launch_bounds__(SK_THREADS) void sk_dq_kernel(SkParams P) {
   float qf[HD / 4], df[HD / 4];
   sk_frag<T, HD>(static_cast<const T*>(P.q) + b * P.qs_b + h * P.qs_h, P.qs_t, i, live, P.hd, kg, qf);
   sk_frag<T, HD>(static_cast<const T*>(P.dout) + b * P.ds_b + h * P.ds_h, P.ds_t, i, live, P.hd, kg, df);
-  const T* o = static_cast<const T*>(P.o) + b * P.os_b + h * P.os_h + i * P.os_t;
-  float dd = 0.f;
+  // D, as the diagonal of dout . out
+  const int only = live ? sk_only_key(P, p) : -1;
+  const int64_t at = only < 0 ? b * P.os_b + h * P.os_h + i * P.os_t : only * P.vs_t;
+  const T* o = only < 0 ? static_cast<const T*>(P.o) : v;
+  f32x4_t d4 = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int s = 0; s < HD / 4; ++s)
-    if (live && 4 * s + kg < P.hd) dd = fmaf(df[s], sk_ld(o, 4 * s + kg), dd);
-  dd = sum_rows4(dd);
+  for (int s = 0; s < HD / 4; ++s) {
+    float x = 0.f;
+    if (live && 4 * s + kg < P.hd) {
+      x = sk_ld(o, at + 4 * s + kg);
+      if (sizeof(T) == 2 && P.olo && only < 0) x += bf16_to_f32(static_cast<const bf16_t*>(P.olo)[at + 4 * s + kg]);
+    }
+    d4 = mfma4(x, df[s], d4);
+  }
+  const float dd = sk_diagonal(d4, r, kg);
   if (i < P.Tq && kg == 0 && part == 0 && blockIdx.z == 0) P.dd[stat] = dd;
   const float lse = live ? P.lse[stat] : INFINITY, sl2 = P.scale * SK_LOG2E;
   f32x4_t acc[HD / 16];
@@ -413,7 +436,7 @@ __global__ __launch_bounds__(64) void sk_join_kernel(SkParams P) {
       const float* p = sk_part_row(P, z, b, h, i);
       x = FWD ? fmaf(p[d], __builtin_amdgcn_exp2f(p[last] - ref), x) : x + p[d];
     }
-    if constexpr (FWD) sk_st(static_cast<T*>(P.o) + b * P.os_b + h * P.os_h + i * P.os_t + d, x * inv);
+    if constexpr (FWD) sk_out<T>(P, b * P.os_b + h * P.os_h + i * P.os_t + d, x * inv);
     else sk_st(static_cast<T*>(P.dq) + row * P.hd + d, x);
   }
 }
@@ -598,8 +621,8 @@ FSI_API int fsi_sink_attn(const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_
                           int64_t ks_h, int64_t ks_t, const void* v, int64_t vs_b, int64_t vs_h, int64_t vs_t,
                           int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t head_dim, int64_t window,
                           int64_t sinks, const int32_t* lengths, float scale, int dtype, void* out, int64_t os_b,
-                          int64_t os_h, int64_t os_t, float* lse, void* workspace, size_t workspace_bytes,
-                          void* stream) {
+                          int64_t os_h, int64_t os_t, void* out_lo, float* lse, void* workspace,
+                          size_t workspace_bytes, void* stream) {
   using namespace fsi_host;
   const int c = sk_check("sink_attn", B, Hq, Hkv, Tq, Tk, head_dim, window, sinks, dtype);
   if (c != FSI_OK || B == 0 || Tq == 0) return c;
@@ -609,6 +632,7 @@ FSI_API int fsi_sink_attn(const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_
                 FSI_ERR_WORKSPACE, "sink_attn: workspace %zu < %zu bytes (or misaligned)", workspace_bytes, need);
   SkParams P = sk_params(q, qs_b, qs_h, qs_t, k, ks_b, ks_h, ks_t, v, vs_b, vs_h, vs_t, out, os_b, os_h, os_t, B, Hq,
                          Hkv, Tq, Tk, head_dim, window, sinks, lengths, scale);
+  P.olo = dtype == FSI_DTYPE_BF16 ? out_lo : nullptr;
   P.lse = lse;
   P.kpart = static_cast<float*>(workspace);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -646,8 +670,8 @@ FSI_API size_t fsi_sink_attn_bwd_workspace_size(int64_t B, int64_t Hq, int64_t H
 
 FSI_API int fsi_sink_attn_bwd(const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_t, const void* k, int64_t ks_b,
                               int64_t ks_h, int64_t ks_t, const void* v, int64_t vs_b, int64_t vs_h, int64_t vs_t,
-                              const void* out, int64_t os_b, int64_t os_h, int64_t os_t, const void* dout, int64_t ds_b,
-                              int64_t ds_h, int64_t ds_t, const float* lse, int64_t B, int64_t Hq, int64_t Hkv,
+                              const void* out, int64_t os_b, int64_t os_h, int64_t os_t, const void* out_lo,
+                              const void* dout, int64_t ds_b, int64_t ds_h, int64_t ds_t, const float* lse, int64_t B, int64_t Hq, int64_t Hkv,
                               int64_t Tq, int64_t Tk, int64_t head_dim, int64_t window, int64_t sinks,
                               const int32_t* lengths, float scale, int dtype, void* dq, void* dk, void* dv,
                               void* workspace, size_t workspace_bytes, void* stream) {
@@ -661,6 +685,7 @@ FSI_API int fsi_sink_attn_bwd(const void* q, int64_t qs_b, int64_t qs_h, int64_t
                 FSI_ERR_WORKSPACE, "sink_attn_bwd: workspace %zu < %zu bytes (or misaligned)", workspace_bytes, need);
   SkParams P = sk_params(q, qs_b, qs_h, qs_t, k, ks_b, ks_h, ks_t, v, vs_b, vs_h, vs_t, out, os_b, os_h, os_t, B, Hq,
                          Hkv, Tq, Tk, head_dim, window, sinks, lengths, scale);
+  P.olo = dtype == FSI_DTYPE_BF16 ? const_cast<void*>(out_lo) : nullptr;
   P.dout = dout;
   P.ds_b = ds_b;
   P.ds_h = ds_h;

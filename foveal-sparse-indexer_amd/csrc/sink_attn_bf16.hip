@@ -4,11 +4,13 @@
 //
 // The score tiles are formed transposed (keys as rows), so a lane's accumulators hold 4 keys
 // times the tiles of one query: the softmax reduces inside the lane and over 4 lanes, and P^T
-// (dS^T) is already the next product's operand.  P and dS are rounded once to bf16 for those
-// products (8 bits; a sum over many keys averages their roundings out, and the output is rounded
-// to 8 bits as well); the output's denominator is the sum of the same rounded P, formed by one
-// more MFMA against ones, so that P's rounding leaves no bias.  The denominator that the backward
-// takes (lse) is the sum before rounding, which forms P again to fp32 precision.
+// (dS^T) is already the next product's operand.  P and (but for few tiles, sb_fine) dS are
+// rounded once to bf16 for those products (8 bits, as the outputs themselves are rounded); the
+// output's denominator is the sum of the same rounded P, formed by one more MFMA against ones, so
+// that P's rounding leaves no bias.  The denominator that the backward takes (lse) is the sum
+// before rounding, which forms P again to fp32 precision, and D = dout . out takes out with the
+// remainder of its rounding: with out alone, rows of few keys have dq and dk up to 3.6e-3 of
+// their norm off, with it 2.4e-3, and 1.75e-3 with dS in two terms (their own rounding: 1.66e-3).
 #include <algorithm>
 #include <type_traits>
 
@@ -30,6 +32,17 @@ __device__ __forceinline__ void sb_frag(const bf16_t* base, int64_t rs, int row,
   for (int s = 0; s < HD / 32; ++s) {
     const u32x4_t x = *reinterpret_cast<const u32x4_t*>(base + row * rs + 32 * s + 8 * kg);
     f[s] = ok ? x : u32x4_t{0u, 0u, 0u, 0u};
+  }
+}
+
+// 8 values, as bf16 and, LO, what that rounding took from them
+template <bool LO>
+__device__ __forceinline__ void sb_round(const f32x4_t& a, const f32x4_t& b, u32x4_t& hi, u32x4_t& lo) {
+  const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    hi[w] = bf_cvt2(x[2 * w], x[2 * w + 1]);
+    if (LO) lo[w] = bf_cvt2(x[2 * w] - lo_bf16(hi[w]), x[2 * w + 1] - hi_bf16(hi[w]));
   }
 }
 
@@ -209,11 +222,18 @@ __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_fwd_kernel(SkPar
       continue;
     }
     const float l = lsum[i][0], inv = l == 0.f ? 0.f : 1.f / l;
-    bf16_t* o = static_cast<bf16_t*>(P.o) + b * P.os_b + h * P.os_h + qi * P.os_t + 4 * kg;
+    const int64_t at = b * P.os_b + h * P.os_h + qi * P.os_t + 4 * kg;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-      *reinterpret_cast<u32x2_t*>(o + 16 * dt) =
-          u32x2_t{bf_cvt2(acc[i][dt][0] * inv, acc[i][dt][1] * inv), bf_cvt2(acc[i][dt][2] * inv, acc[i][dt][3] * inv)};
+    for (int dt = 0; dt < DT; ++dt) {
+      const f32x4_t x = acc[i][dt] * inv;
+      const u32x2_t w = u32x2_t{bf_cvt2(x[0], x[1]), bf_cvt2(x[2], x[3])};
+      *reinterpret_cast<u32x2_t*>(static_cast<bf16_t*>(P.o) + at + 16 * dt) = w;
+      if (LSE && P.olo) {
+        const u32x2_t e = u32x2_t{bf_cvt2(x[0] - lo_bf16(w[0]), x[1] - hi_bf16(w[0])),
+                                  bf_cvt2(x[2] - lo_bf16(w[1]), x[3] - hi_bf16(w[1]))};
+        *reinterpret_cast<u32x2_t*>(static_cast<bf16_t*>(P.olo) + at + 16 * dt) = e;
+      }
+    }
     if (LSE && kg == 0)
       P.lse[(static_cast<int64_t>(b) * P.Hq + h) * P.Tq + qi] = l == 0.f ? INFINITY : m[i] + __log2f(l_full[i]);
   }
@@ -223,7 +243,7 @@ __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_fwd_kernel(SkPar
 // dQ, and D for the key kernel.  A workgroup of 4 waves is HPW query heads of one KV head at
 // 64 * 2 / HPW queries; a wave is one head's 32 queries over 32 keys at a time.
 // ---------------------------------------------------------------------------
-template <int HD, int HPW>
+template <int HD, int HPW, bool FINE>
 __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_dq_kernel(SkParams P) {
   constexpr int KS = HD / 32, DT = HD / 16, TB = sab_tile_bytes<HD>();
   constexpr int QW = SB_WAVES / HPW * 32;
@@ -258,17 +278,18 @@ __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_dq_kernel(SkPara
     sb_frag<HD>(static_cast<const bf16_t*>(P.q) + b * P.qs_b + h * P.qs_h, P.qs_t, ql, live, kg, q[i]);
     sb_frag<HD>(static_cast<const bf16_t*>(P.dout) + b * P.ds_b + h * P.ds_h, P.ds_t, ql, live, kg,
                 gr[i]);
-    u32x4_t of[KS];
-    sb_frag<HD>(static_cast<const bf16_t*>(P.o) + b * P.os_b + h * P.os_h, P.os_t, ql, live, kg, of);
-    float d = 0.f;
+    u32x4_t of[KS], ol[KS];
+    const int64_t head = b * P.os_b + h * P.os_h;
+    const int only = live ? sk_only_key(P, off + qi) : -1;
+    sb_frag<HD>(only < 0 ? static_cast<const bf16_t*>(P.o) + head : v, only < 0 ? P.os_t : P.vs_t, only < 0 ? ql : only,
+                live, kg, of);
+    sb_frag<HD>(static_cast<const bf16_t*>(P.olo ? P.olo : P.o) + head, P.os_t, ql, live && P.olo && only < 0, kg, ol);
+    f32x4_t d = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
+    for (int s = 0; s < KS; ++s) d = mfma16x16x32(of[s], gr[i][s], d);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        d = fmaf(lo_bf16(gr[i][s][w]), lo_bf16(of[s][w]), d);
-        d = fmaf(hi_bf16(gr[i][s][w]), hi_bf16(of[s][w]), d);
-      }
-    dd[i] = sum_rows4(d);
+    for (int s = 0; s < KS; ++s) d = mfma16x16x32(ol[s], gr[i][s], d);
+    dd[i] = sk_diagonal(d, r, kg);
     lse[i] = live ? P.lse[stat + qi] : INFINITY;
     hi[i] = live ? off + qi : -1;
     if (qi < P.Tq && kg == 0 && blockIdx.z == 0) P.dd[stat + qi] = dd[i];
@@ -326,16 +347,17 @@ __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_dq_kernel(SkPara
 #pragma unroll
           for (int j = 0; j < 4; ++j)  // dS^T
             dp[i][t][j] = __builtin_amdgcn_exp2f(fmaf(st[i][t][j], sl2, -lse[i])) * (dp[i][t][j] - dd[i]);
-      u32x4_t ds[2];
+      u32x4_t ds[2], dl[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) ds[i][w] = bf_cvt2(dp[i][w >> 1][2 * (w & 1)], dp[i][w >> 1][2 * (w & 1) + 1]);
+      for (int i = 0; i < 2; ++i) sb_round<FINE>(dp[i][0], dp[i][1], ds[i], dl[i]);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const u32x4_t a = sab_trow<HD>(smem, tr_off + at, dt, 0);
-        acc[0][dt] = mfma16x16x32(a, ds[0], acc[0][dt]);
-        acc[1][dt] = mfma16x16x32(a, ds[1], acc[1][dt]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (FINE) acc[i][dt] = mfma16x16x32(a, dl[i], acc[i][dt]);
+          acc[i][dt] = mfma16x16x32(a, ds[i], acc[i][dt]);
+        }
       }
     }
     __syncthreads();
@@ -364,7 +386,7 @@ __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_dq_kernel(SkPara
 // queries; the two query halves' sums meet in LDS at the end.
 // The first S.tiles * S.parts workgroups of a KV head are the split sink tiles' (SkSinkSplit).
 // ---------------------------------------------------------------------------
-template <int HD>
+template <int HD, bool FINE>
 __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_dkv_kernel(SkParams P, SkSinkSplit S) {
   constexpr int KS = HD / 32, DT = HD / 16, TB = sab_tile_bytes<HD>();
   constexpr int STAGE = 2 * TB + 2 * AB_T * 4;    // Q, dout, then lse and D of the rows
@@ -469,14 +491,12 @@ __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_dkv_kernel(SkPar
             s[kt][qt][e] = p;
           }
       }
-      u32x4_t ph[2], dh[2];
+      u32x4_t ph[2], dh[2], dl[2];
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          ph[kt][w] = bf_cvt2(s[kt][w >> 1][2 * (w & 1)], s[kt][w >> 1][2 * (w & 1) + 1]);
-          dh[kt][w] = bf_cvt2(dp[kt][w >> 1][2 * (w & 1)], dp[kt][w >> 1][2 * (w & 1) + 1]);
-        }
+      for (int kt = 0; kt < 2; ++kt) {
+        sb_round<false>(s[kt][0], s[kt][1], ph[kt], dl[kt]);
+        sb_round<FINE>(dp[kt][0], dp[kt][1], dh[kt], dl[kt]);
+      }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const u32x4_t ad = sab_trow<HD>(smem, tr_off + cur, dt, TB);
@@ -484,6 +504,7 @@ __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_dkv_kernel(SkPar
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
           dva[kt][dt] = mfma16x16x32(ad, ph[kt], dva[kt][dt]);
+          if (FINE) dka[kt][dt] = mfma16x16x32(aq, dl[kt], dka[kt][dt]);
           dka[kt][dt] = mfma16x16x32(aq, dh[kt], dka[kt][dt]);
         }
       }
@@ -536,7 +557,7 @@ bool sb_takes(const SkParams& P, int dtype, bool backward) {
   };
   return dtype == FSI_DTYPE_BF16 && (P.hd == 64 || P.hd == 128 || P.hd == 256) && P.scale > 0.f && P.Tq > 0 &&
          rows(P.q, P.qs_b, P.qs_h, P.qs_t) && rows(P.k, P.ks_b, P.ks_h, P.ks_t) && rows(P.v, P.vs_b, P.vs_h, P.vs_t) &&
-         rows(P.o, P.os_b, P.os_h, P.os_t) &&
+         rows(P.o, P.os_b, P.os_h, P.os_t) && reinterpret_cast<uintptr_t>(P.olo) % 16 == 0 &&
          (!backward || (rows(P.dout, P.ds_b, P.ds_h, P.ds_t) &&
                         (reinterpret_cast<uintptr_t>(P.dq) | reinterpret_cast<uintptr_t>(P.dk) |
                          reinterpret_cast<uintptr_t>(P.dv)) % 8 == 0));
@@ -576,24 +597,39 @@ void sb_forward(const SkParams& P, hipStream_t st) {
   else run(std::integral_constant<int, 64>{});
 }
 
+// Up to this many key tiles a launch leaves most of the card idle, and dS enters its products as two
+// bf16 terms: with few keys a row, rounding it once is most of dq's and dk's error (2.4e-3 of their norm
+// against 1.7e-3, which is their own rounding).  us of the backward, one term / two: heads of 64, 8
+// heads of 512 tokens (64 tiles) 27.8 / 29.8; heads of 128, (4, 4 heads, 27) 13.6 / 14.6, 8 heads of 512
+// 39.7 / 46.7.  Beyond, the product would be paid for in full: (1, 16 / 4 heads, 2048, 128) 151 / 190.
+constexpr int SB_FINE_TILES = 64;
+static bool sb_fine(const SkParams& P) {
+  return SB_FINE_TILES >= static_cast<int64_t>(P.B) * P.Hkv * ((P.Tk + SK_T - 1) / SK_T);
+}
+
 void sb_backward(const SkParams& P, const SkSinkSplit& S, hipStream_t st) {
-  auto run = [&](auto hd) {
+  auto run = [&](auto hd, auto fine) {
     constexpr int HD = decltype(hd)::value;
+    constexpr bool FINE = decltype(fine)::value;
     auto launch = [&](auto heads) {
       constexpr int HPW = decltype(heads)::value, QW = SB_WAVES / HPW * 32;
       const dim3 grid(static_cast<unsigned>((P.Tq + QW - 1) / QW * (P.Hq / HPW)), static_cast<unsigned>(P.B),
                       P.ksplit);
-      sb_dq_kernel<HD, HPW><<<grid, SB_THREADS, 0, st>>>(P);
+      sb_dq_kernel<HD, HPW, FINE><<<grid, SB_THREADS, 0, st>>>(P);
     };
     if (sb_heads(P, 2) == 2) launch(std::integral_constant<int, 2>{});
     else launch(std::integral_constant<int, 1>{});
     const unsigned tiles = static_cast<unsigned>((P.Tk + SK_T - 1) / SK_T + S.tiles * S.parts);
-    sb_dkv_kernel<HD><<<dim3(tiles * static_cast<unsigned>(P.Hkv), static_cast<unsigned>(P.B), P.hsplit), SB_THREADS, 0,
-                        st>>>(P, S);
+    sb_dkv_kernel<HD, FINE><<<dim3(tiles * static_cast<unsigned>(P.Hkv), static_cast<unsigned>(P.B), P.hsplit),
+                              SB_THREADS, 0, st>>>(P, S);
   };
-  if (P.hd == 256) run(std::integral_constant<int, 256>{});
-  else if (P.hd == 128) run(std::integral_constant<int, 128>{});
-  else run(std::integral_constant<int, 64>{});
+  auto by_width = [&](auto fine) {
+    if (P.hd == 256) run(std::integral_constant<int, 256>{}, fine);
+    else if (P.hd == 128) run(std::integral_constant<int, 128>{}, fine);
+    else run(std::integral_constant<int, 64>{}, fine);
+  };
+  if (sb_fine(P)) by_width(std::true_type{});
+  else by_width(std::false_type{});
 }
 
 }  // namespace fsi_sink

@@ -49,19 +49,22 @@ def _out_like(q: Tensor) -> Tensor:
     return q.new_empty((B, Tq, Hq, hd)).transpose(1, 2)
 
 
-def _fwd_fake(q, k, v, lengths, window, sinks, scale, want_lse):
-    return _out_like(q), q.new_empty(q.shape[:3] if want_lse else (0,), dtype=torch.float32)
+def _fwd_fake(q, k, v, lengths, window, sinks, scale, grad):
+    lo = _out_like(q) if grad and q.dtype == torch.bfloat16 else q.new_empty((0,))
+    return _out_like(q), q.new_empty(q.shape[:3] if grad else (0,), dtype=torch.float32), lo
 
 
 @_lib.fsi_op("sink_window_attention", _fwd_fake)
 def _fwd_op(q: Tensor, k: Tensor, v: Tensor, lengths: Optional[Tensor], window: int, sinks: int, scale: float,
-            want_lse: bool) -> Tuple[Tensor, Tensor]:
-    """fsi_sink_attn: (out (B, Hq, Tq, hd), lse (B, Hq, Tq) or empty)."""
+            grad: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    """fsi_sink_attn: (out (B, Hq, Tq, hd), and for the backward lse (B, Hq, Tq) and, bf16, out's
+    rounding remainder; else empty)."""
     dev = q.device
     q, k, v = _rows(q), _rows(k), _rows(v)
     B, Hq, Tq, hd = q.shape
     out = _out_like(q)
-    lse = torch.empty((B, Hq, Tq) if want_lse else (0,), dtype=torch.float32, device=dev)
+    lse = torch.empty((B, Hq, Tq) if grad else (0,), dtype=torch.float32, device=dev)
+    lo = _out_like(q) if grad and q.dtype == torch.bfloat16 else q.new_empty((0,))
     L = _lib.lib()
     Hkv, Tk = k.shape[1], k.shape[2]
     need = L.fsi_sink_attn_workspace_size(B, Hq, Hkv, Tq, Tk, hd, window, sinks)
@@ -70,21 +73,22 @@ def _fwd_op(q: Tensor, k: Tensor, v: Tensor, lengths: Optional[Tensor], window: 
         st = L.fsi_sink_attn(
             q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], B, Hq, Hkv,
             Tq, Tk, hd, window, sinks, _lib.ptr(lengths), scale, _lib.dtype_code(q.dtype, _WHAT), out.data_ptr(),
-            *out.stride()[:3], lse.data_ptr() if want_lse else None, _lib.ptr(ws), need, _lib.stream_handle(dev))
+            *out.stride()[:3], lo.data_ptr() if lo.numel() else None, lse.data_ptr() if grad else None, _lib.ptr(ws), need,
+            _lib.stream_handle(dev))
     _lib.check(st, _WHAT)
-    return out, lse
+    return out, lse, lo
 
 
-def _bwd_fake(q, k, v, out, dout, lse, lengths, window, sinks, scale):
+def _bwd_fake(q, k, v, out, lo, dout, lse, lengths, window, sinks, scale):
     return tuple(torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
 
 
 @_lib.fsi_op("sink_window_attention_bwd", _bwd_fake)
-def _bwd_op(q: Tensor, k: Tensor, v: Tensor, out: Tensor, dout: Tensor, lse: Tensor, lengths: Optional[Tensor],
-            window: int, sinks: int, scale: float) -> Tuple[Tensor, Tensor, Tensor]:
+def _bwd_op(q: Tensor, k: Tensor, v: Tensor, out: Tensor, lo: Tensor, dout: Tensor, lse: Tensor,
+            lengths: Optional[Tensor], window: int, sinks: int, scale: float) -> Tuple[Tensor, Tensor, Tensor]:
     """fsi_sink_attn_bwd: contiguous (dq, dk, dv) of the operands' dtype."""
     dev = q.device
-    q, k, v, out, dout = (_rows(t) for t in (q, k, v, out, dout))
+    q, k, v, dout = (_rows(t) for t in (q, k, v, dout))
     B, Hq, Tq, hd = q.shape
     Hkv, Tk = k.shape[1], k.shape[2]
     dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
@@ -94,7 +98,7 @@ def _bwd_op(q: Tensor, k: Tensor, v: Tensor, out: Tensor, dout: Tensor, lse: Ten
     with _lib.device_guard(dev):
         st = L.fsi_sink_attn_bwd(
             q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3],
-            out.data_ptr(), *out.stride()[:3], dout.data_ptr(), *dout.stride()[:3], lse.data_ptr(), B, Hq, Hkv, Tq,
+            out.data_ptr(), *out.stride()[:3], lo.data_ptr() if lo.numel() else None, dout.data_ptr(), *dout.stride()[:3], lse.data_ptr(), B, Hq, Hkv, Tq,
             Tk, hd, window, sinks, _lib.ptr(lengths), scale, _lib.dtype_code(q.dtype, _WHAT), dq.data_ptr(),
             dk.data_ptr(), dv.data_ptr(), _lib.ptr(ws), need, _lib.stream_handle(dev))
     _lib.check(st, f"{_WHAT} backward")
@@ -103,20 +107,21 @@ def _bwd_op(q: Tensor, k: Tensor, v: Tensor, out: Tensor, dout: Tensor, lse: Ten
 
 class _SinkAttnFn(torch.autograd.Function):
     """sink_window_attention with gradients for q, k and v: the forward keeps each row's softmax
-    denominator, and the backward forms P again from it tile by tile."""
+    denominator and (bf16) what rounding took from its output, and the backward forms P again tile by
+    tile."""
 
     @staticmethod
     def forward(ctx, q, k, v, lengths, window, sinks, scale):
-        out, lse = _fwd_op(q, k, v, lengths, window, sinks, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, lengths)
+        out, lse, lo = _fwd_op(q, k, v, lengths, window, sinks, scale, True)
+        ctx.save_for_backward(q, k, v, out, lo, lse, lengths)
         ctx.meta = (window, sinks, scale)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, lengths = ctx.saved_tensors
-        grads = _bwd_op(q, k, v, out, dout.to(q.dtype), lse, lengths, *ctx.meta)
+        q, k, v, out, lo, lse, lengths = ctx.saved_tensors
+        grads = _bwd_op(q, k, v, out, lo, dout.to(q.dtype), lse, lengths, *ctx.meta)
         return (*grads, None, None, None, None)
 
 

@@ -659,6 +659,9 @@ FSI_API int fsi_sparse_attn_bwd(const void* q, int64_t qs_b, int64_t qs_h, int64
  * runs on bf16 MFMA, everything else on fp32 MFMA.
  * lse (B, Hq, Tq) fp32 (null: not wanted): log2 of each query's softmax denominator in
  * units of scale log2(e) q.k, which the backward takes; +inf for a query without keys.
+ * out_lo (null: not wanted; fp32: not written): bf16 array laid out as out, what rounding took
+ * from it.  With it the backward's dout . out keeps 16 bits; without it dq and dk of few
+ * keys are as coarse as out.
  *
  * The backward writes contiguous dq (B, Hq, Tq, head_dim), dk and dv (B, Hkv, Tk, head_dim)
  * of dtype, dk and dv summed over the query heads of a KV head in fp32, in a fixed order.
@@ -670,15 +673,15 @@ FSI_API int fsi_sink_attn(const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_
                           int64_t ks_h, int64_t ks_t, const void* v, int64_t vs_b, int64_t vs_h, int64_t vs_t,
                           int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t head_dim, int64_t window,
                           int64_t sinks, const int32_t* lengths, float scale, int dtype, void* out, int64_t os_b,
-                          int64_t os_h, int64_t os_t, float* lse, void* workspace, size_t workspace_bytes,
-                          void* stream);
+                          int64_t os_h, int64_t os_t, void* out_lo, float* lse, void* workspace,
+                          size_t workspace_bytes, void* stream);
 
 FSI_API size_t fsi_sink_attn_bwd_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t Tk,
                                                 int64_t head_dim, int64_t window, int64_t sinks);
 FSI_API int fsi_sink_attn_bwd(const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_t, const void* k, int64_t ks_b,
                               int64_t ks_h, int64_t ks_t, const void* v, int64_t vs_b, int64_t vs_h, int64_t vs_t,
-                              const void* out, int64_t os_b, int64_t os_h, int64_t os_t, const void* dout, int64_t ds_b,
-                              int64_t ds_h, int64_t ds_t, const float* lse, int64_t B, int64_t Hq, int64_t Hkv,
+                              const void* out, int64_t os_b, int64_t os_h, int64_t os_t, const void* out_lo,
+                              const void* dout, int64_t ds_b, int64_t ds_h, int64_t ds_t, const float* lse, int64_t B, int64_t Hq, int64_t Hkv,
                               int64_t Tq, int64_t Tk, int64_t head_dim, int64_t window, int64_t sinks,
                               const int32_t* lengths, float scale, int dtype, void* dq, void* dk, void* dv,
                               void* workspace, size_t workspace_bytes, void* stream);

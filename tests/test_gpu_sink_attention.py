@@ -313,3 +313,40 @@ def test_prompt_then_tokens(fsi, dev, fmt):
                                          None, 1 / math.sqrt(hd), *UNIT[BF16])
             for got in (tok, ref):
                 assert ((got.double().cpu() - want[0][:, :, 0]).abs() <= tol[0][:, :, 0]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("hd", [64, 80, 128, 256])
+@pytest.mark.parametrize("Hq,Hkv,Tq,Tk,window,sinks", [
+    (2, 1, 1, 1, 1, 0), (3, 3, 1, 1, 9, 4), (4, 2, 100, 130, 1, 0), (4, 2, 100, 130, 0, 1), (2, 2, 300, 300, 1, 0),
+])
+def test_a_single_key_has_no_score_gradient(fsi, dev, dtype, hd, Hq, Hkv, Tq, Tk, window, sinks):
+    """Softmax over one key is 1 whatever its score: dq and dk are 0 to the bit."""
+    q, k, v, dout = _inputs(2, Hq, Hkv, Tq, Tk, hd, dtype, seed=hd + Tq)
+    got = _run(fsi, dev, q * 3, k, v, dout * 100, window=window, sinks=sinks)
+    assert (got[1] == 0).all() and (got[2] == 0).all()
+    _check(got, *oracle.attention(q * 3, k, v, dout * 100, window, sinks, None, 1 / math.sqrt(hd), *UNIT[dtype]))
+
+
+@pytest.mark.parametrize("hd", [64, 80, 128])
+def test_the_output_is_kept_to_sixteen_bits_for_the_backward(fsi, dev, hd):
+    """out and what rounding took from it: at most half a step, which is at most 2^-8 of out (rounding
+    the remainder itself may bring it to exactly half a step, so that their sum need not round to out),
+    and where P is not rounded (80) the sum is the value to 2^-16 of it and the result's fp32 error."""
+    q, k, v, dout = _inputs(2, 4, 2, 150, 150, hd, BF16, seed=hd)
+    out, lse, lo = torch.ops.fsi.sink_window_attention(
+        q.to(dev), k.to(dev), v.to(dev), None, 40, 3, 1 / math.sqrt(hd), True)
+    both = out.double() + lo.double()
+    assert (lo.double().abs() <= 2.0**-8 * out.double().abs()).all() and (lo != 0).any()
+    if hd == 80:
+        want, _ = oracle.attention(q, k, v, dout, 40, 3, None, 1 / math.sqrt(hd), *UNIT[BF16])
+        _, tol = oracle.attention(q, k, v, dout, 40, 3, None, 1 / math.sqrt(hd), *UNIT[F32])
+        assert ((both.cpu() - want[0]).abs() <= tol[0] + 2.0**-16 * want[0].abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+def test_scales_of_either_sign(fsi, dev, dtype, scale):
+    q, k, v, dout = _inputs(1, 4, 2, 130, 130, 64, dtype, seed=12)
+    got = _run(fsi, dev, q, k, v, dout, window=50, sinks=3, scale=scale)
+    _check(got, *oracle.attention(q, k, v, dout, 50, 3, None, scale, *UNIT[dtype]))

@@ -78,10 +78,10 @@ def test_sink_attention_errors(fsi):
 
     def fwd(q=_ptr(1), B=1, Hq=4, Hkv=2, Tq=3, Tk=5, hd=64, window=2, sinks=1, dtype=1):
         return L.fsi_sink_attn(q, 1, 1, 1, _ptr(2), 1, 1, 1, _ptr(3), 1, 1, 1, B, Hq, Hkv, Tq, Tk, hd, window, sinks,
-                               None, 1.0, dtype, _ptr(4), 1, 1, 1, None, None, 0, None)
+                               None, 1.0, dtype, _ptr(4), 1, 1, 1, None, None, None, 0, None)
 
     def bwd(q=_ptr(1), Tq=3, Tk=5, hd=64, dtype=1, ws=None, nbytes=0, dk=_ptr(8)):
-        return L.fsi_sink_attn_bwd(q, 1, 1, 1, _ptr(2), 1, 1, 1, _ptr(3), 1, 1, 1, _ptr(4), 1, 1, 1, _ptr(5), 1, 1, 1,
+        return L.fsi_sink_attn_bwd(q, 1, 1, 1, _ptr(2), 1, 1, 1, _ptr(3), 1, 1, 1, _ptr(4), 1, 1, 1, None, _ptr(5), 1, 1, 1,
                                    _ptr(6), 1, 4, 2, Tq, Tk, hd, 2, 1, None, 1.0, dtype, _ptr(7), dk, _ptr(9), ws,
                                    nbytes, None)
 

@@ -27,10 +27,11 @@ def test_registered_and_fake_shapes(fsi):
         o = ops.decode_attention_sinks(q3, pool, pool, 2, table, 10, 10, 2, None, 70, 64, 4, None, None, 0, 0.1)
         assert o.shape == q3.shape and o.dtype == BF16
         q, kk = _fake(2, 8, 100, 64), _fake(2, 2, 130, 64)
-        o, lse = ops.sink_window_attention(q, kk, kk, None, 30, 4, 0.125, True)
+        o, lse, lo = ops.sink_window_attention(q, kk, kk, None, 30, 4, 0.125, True)
         assert o.shape == q.shape and o.transpose(1, 2).is_contiguous() and lse.shape == (2, 8, 100)
+        assert lo.shape == o.shape and lo.stride() == o.stride()
         assert ops.sink_window_attention(q, kk, kk, None, 30, 4, 0.125, False)[1].numel() == 0
-        grads = ops.sink_window_attention_bwd(q, kk, kk, o, o, lse, None, 30, 4, 0.125)
+        grads = ops.sink_window_attention_bwd(q, kk, kk, o, lo, o, lse, None, 30, 4, 0.125)
         assert [g.shape for g in grads] == [q.shape, kk.shape, kk.shape] and all(g.is_contiguous() for g in grads)
 
 
@@ -50,7 +51,7 @@ def test_opcheck(fsi, dev, i):
     ops = torch.ops.fsi
     c = _held(fsi, dev, "mxfp4")
     q, kv = _randn(2, 4, 70, 64, seed=3), _randn(2, 2, 90, 64, seed=4)
-    out, lse = ops.sink_window_attention(q, kv, kv, None, 30, 4, 0.125, True)
+    out, lse, lo = ops.sink_window_attention(q, kv, kv, None, 30, 4, 0.125, True)
     op, args = [
         (ops.kv_mx_write, (_randn(2, 2, 5, 64, seed=5), _randn(2, 2, 5, 64, seed=6), 2, None, 9, c.page_table,
                            c.max_pages, c.n_phys_pages, c.k_cache, c.v_cache)),
@@ -59,7 +60,7 @@ def test_opcheck(fsi, dev, i):
                                       c.n_phys_pages, 2, None, 120, 30, 4, None, None, 0, 0.125)),
         (ops.sink_window_attention, (q, kv, kv, torch.tensor([90, 80], dtype=torch.int32, device=dev), 30, 4, 0.125,
                                      True)),
-        (ops.sink_window_attention_bwd, (q, kv, kv, out, _randn(2, 4, 70, 64, seed=8), lse, None, 30, 4, 0.125)),
+        (ops.sink_window_attention_bwd, (q, kv, kv, out, lo, _randn(2, 4, 70, 64, seed=8), lse, None, 30, 4, 0.125)),
     ][i]
     torch.library.opcheck(op, args, test_utils=("test_schema", "test_faketensor", "test_aot_dispatch_dynamic"))
 
