@@ -220,6 +220,8 @@ class FovealKVCache:
         if isinstance(start, Tensor):
             if self.kv_format is None:
                 raise TypeError(f"{what}: per-sequence start positions need a cache with a kv_format")
+            if start.is_floating_point() or start.dtype == torch.bool:
+                raise TypeError(f"{what}: start positions must be integers, got {start.dtype}")
             rows = start.to(device=self.k_cache.device, dtype=torch.int32).reshape(-1).contiguous()
             if rows.numel() != B:
                 raise ValueError(f"{what}: {rows.numel()} start positions for {B} sequences")
@@ -283,6 +285,7 @@ class FovealKVCache:
             return self.k_cache[sel, :, :n].clone(), self.v_cache[sel, :, :n].clone()
         rows = self.page_table[batch] if batch is not None else self.page_table
         if self.kv_format is not None:
+            _lib.require_gpu(self.k_cache, what="FovealKVCache.to_dense")
             return _kv_mx_read_op(self.k_cache, self.v_cache, rows.contiguous(), _lib.KV_FORMATS[self.kv_format],
                                   self.num_kv_heads, n, self.head_dim, self.max_pages, self.n_phys_pages,
                                   _lib.dtype_code(self.dtype, "FovealKVCache.to_dense"))

@@ -68,7 +68,8 @@ __device__ __forceinline__ void mx_ld8(const T* p, bool vec, float (&x)[8]) {
 // dim pair e (2 bits / 8 bytes each), the scale byte returned.  v_cvt_scalef32_pk_{fp4,fp8}_f32
 // divides by the scale and rounds to the nearest element, ties to even; the clamp before it takes
 // what lies above the largest.  (Rounding in integer code instead, 10 instructions an element, made
-// the vector units the bound: 8192-token prompts of 4 sequences written in 44 against 31 us, read back in 42 against 26.)
+// the vector units the bound: 8192-token prompts of 4 sequences written in 44 against 31 us, read
+// back in 42 against 26.)
 template <int FMT>
 __device__ __forceinline__ int mx_quantise8(const float (&x)[8], uint32_t (&pair)[4]) {
   uint32_t amax = 0;
@@ -103,8 +104,10 @@ __device__ __forceinline__ void mx_widen8(const uint32_t (&c)[4], int byte, T* d
     u32x4_t w;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if constexpr (FMT == FMT_FP4) w[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[e], scale, 0));
-      else w[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[e], scale, false));
+      if constexpr (FMT == FMT_FP4)
+        w[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[e], scale, 0));
+      else
+        w[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[e], scale, false));
       w[e] = nan ? 0x7fc07fc0u : w[e];
     }
     *reinterpret_cast<u32x4_t*>(dst) = w;

@@ -49,8 +49,10 @@ typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2v_t;
 
 template <int FMT, int SEL>
 __device__ __forceinline__ uint32_t widen(uint32_t w, float s) {
-  if constexpr (FMT == FMT_FP4) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, SEL));
-  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, SEL != 0));
+  if constexpr (FMT == FMT_FP4)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, SEL));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, SEL != 0));
 }
 
 // N consecutive dwords at p (aligned to the largest power of two in 4 N bytes, at most 16), each
@@ -556,7 +558,8 @@ FSI_API int fsi_decode_attn_sinks(const void* q, int dtype, const void* k_pool, 
                 "decode_attn_sinks: format %d", format);
   FSI_CHECK_ARG(dtype == FSI_DTYPE_BF16 || (dtype == FSI_DTYPE_F32 && format != FSI_KV_BF16), FSI_ERR_DTYPE,
                 "decode_attn_sinks: dtype %d (bf16 pages take bf16 queries)", dtype);
-  const bool hd_ok = format == FSI_KV_BF16 ? head_dim == 64 || head_dim == 128 : fsi_kv_mx_block_bytes(head_dim, format) > 0;
+  const bool hd_ok = format == FSI_KV_BF16 ? head_dim == 64 || head_dim == 128
+                                           : fsi_kv_mx_block_bytes(head_dim, format) > 0;
   FSI_CHECK_ARG(hd_ok, FSI_ERR_SHAPE, "decode_attn_sinks: head_dim %lld (bf16 pages 64 or 128, else 64, 96, 128, 256)",
                 (long long)head_dim);
   FSI_CHECK_ARG(B >= 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0, FSI_ERR_SHAPE,

@@ -671,8 +671,9 @@ FSI_API size_t fsi_sink_attn_bwd_workspace_size(int64_t B, int64_t Hq, int64_t H
 FSI_API int fsi_sink_attn_bwd(const void* q, int64_t qs_b, int64_t qs_h, int64_t qs_t, const void* k, int64_t ks_b,
                               int64_t ks_h, int64_t ks_t, const void* v, int64_t vs_b, int64_t vs_h, int64_t vs_t,
                               const void* out, int64_t os_b, int64_t os_h, int64_t os_t, const void* out_lo,
-                              const void* dout, int64_t ds_b, int64_t ds_h, int64_t ds_t, const float* lse, int64_t B, int64_t Hq, int64_t Hkv,
-                              int64_t Tq, int64_t Tk, int64_t head_dim, int64_t window, int64_t sinks,
+                              const void* dout, int64_t ds_b, int64_t ds_h, int64_t ds_t, const float* lse,
+                              int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t head_dim,
+                              int64_t window, int64_t sinks,
                               const int32_t* lengths, float scale, int dtype, void* dq, void* dk, void* dv,
                               void* workspace, size_t workspace_bytes, void* stream) {
   using namespace fsi_host;

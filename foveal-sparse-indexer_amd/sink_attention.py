@@ -73,8 +73,8 @@ def _fwd_op(q: Tensor, k: Tensor, v: Tensor, lengths: Optional[Tensor], window: 
         st = L.fsi_sink_attn(
             q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], B, Hq, Hkv,
             Tq, Tk, hd, window, sinks, _lib.ptr(lengths), scale, _lib.dtype_code(q.dtype, _WHAT), out.data_ptr(),
-            *out.stride()[:3], lo.data_ptr() if lo.numel() else None, lse.data_ptr() if grad else None, _lib.ptr(ws), need,
-            _lib.stream_handle(dev))
+            *out.stride()[:3], lo.data_ptr() if lo.numel() else None, lse.data_ptr() if grad else None, _lib.ptr(ws),
+            need, _lib.stream_handle(dev))
     _lib.check(st, _WHAT)
     return out, lse, lo
 
@@ -89,6 +89,8 @@ def _bwd_op(q: Tensor, k: Tensor, v: Tensor, out: Tensor, lo: Tensor, dout: Tens
     """fsi_sink_attn_bwd: contiguous (dq, dk, dv) of the operands' dtype."""
     dev = q.device
     q, k, v, dout = (_rows(t) for t in (q, k, v, dout))
+    if out.stride(3) != 1 or (lo.numel() and lo.stride() != out.stride()):  # the kernels read both by out's strides
+        out, lo = out.contiguous(), lo.contiguous()
     B, Hq, Tq, hd = q.shape
     Hkv, Tk = k.shape[1], k.shape[2]
     dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
@@ -98,9 +100,10 @@ def _bwd_op(q: Tensor, k: Tensor, v: Tensor, out: Tensor, lo: Tensor, dout: Tens
     with _lib.device_guard(dev):
         st = L.fsi_sink_attn_bwd(
             q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3],
-            out.data_ptr(), *out.stride()[:3], lo.data_ptr() if lo.numel() else None, dout.data_ptr(), *dout.stride()[:3], lse.data_ptr(), B, Hq, Hkv, Tq,
-            Tk, hd, window, sinks, _lib.ptr(lengths), scale, _lib.dtype_code(q.dtype, _WHAT), dq.data_ptr(),
-            dk.data_ptr(), dv.data_ptr(), _lib.ptr(ws), need, _lib.stream_handle(dev))
+            out.data_ptr(), *out.stride()[:3], lo.data_ptr() if lo.numel() else None, dout.data_ptr(),
+            *dout.stride()[:3], lse.data_ptr(), B, Hq, Hkv, Tq, Tk, hd, window, sinks, _lib.ptr(lengths), scale,
+            _lib.dtype_code(q.dtype, _WHAT), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(ws), need,
+            _lib.stream_handle(dev))
     _lib.check(st, f"{_WHAT} backward")
     return dq, dk, dv
 

@@ -355,3 +355,52 @@ def test_module_decodes_from_a_held_cache(fsi, dev, fmt, dtype):
                 u = torch.finfo(dtype).eps / 2
                 tol = 4 * u * (att.abs().float() @ m.out_proj.weight.abs().float().t() + want.abs().float()) + 1e-6
                 assert ((out - want).abs().float() <= tol).all()
+
+
+@pytest.mark.parametrize("fmt,hd,H,n_phys", [("mxfp8", 256, 2, 140000), ("mxfp4", 256, 4, 140000),
+                                              (None, 128, 2, 140000)])
+def test_pages_beyond_32_bit_offsets(fsi, dev, fmt, hd, H, n_phys):
+    """Pools of more than 4 GiB: pages at their end are written, read and attended as those of a small one."""
+    high = torch.tensor([[n_phys - 1, 3, n_phys - 2]], dtype=torch.int32)
+    g = torch.Generator().manual_seed(13)
+    k, v = (torch.randn(1, H, 180, hd, generator=g).to(BF16).to(dev) for _ in range(2))
+    q = torch.randn(1, 2 * H, hd, generator=g).to(BF16).to(dev)
+    got = []
+    for n, table in ((n_phys, high), (8, torch.tensor([[7, 3, 6]], dtype=torch.int32))):
+        c = fsi.FovealKVCache(1, 192, H, hd, 16, 64, dev, BF16, n_phys_pages=n, page_table=table, kv_format=fmt)
+        assert n == 8 or c.k_cache.numel() * c.k_cache.element_size() > 1 << 32
+        c.load_dense(k, v)
+        o = fsi.decode_attention(q, c, pos=179, window=70, remote_pages=torch.tensor([[0]], device=dev),
+                                 remote_counts=torch.tensor([1], device=dev), scale=1 / math.sqrt(hd), sinks=9)
+        got.append((o, *c.to_dense(180)))
+    for a, b in zip(*got):
+        assert torch.equal(a, b) and a.abs().max() > 0
+
+
+def test_two_graphs_replayed_side_by_side(fsi, dev):
+    """Graphs captured on one stream and replayed on two at once have partials of their own."""
+    g = torch.Generator().manual_seed(14)
+    T, hd = 5000, 128
+    c = _cache(fsi, dev, 1, T, 1, hd, BF16, "mxfp4")
+    c.load_dense(*(torch.randn(1, 1, T, hd, generator=g).to(BF16).to(dev) for _ in range(2)))
+    qs = [torch.randn(1, 8, hd, generator=g).to(BF16).to(dev) for _ in range(2)]
+
+    def step(q):
+        return fsi.decode_attention(q, c, pos=T - 1, window=1 << 20, remote_pages=None, remote_counts=None,
+                                    scale=1 / math.sqrt(hd), sinks=4)
+
+    want = [step(q) for q in qs]
+    graphs, held = [], []
+    for q in qs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            held.append(step(q))
+    streams = [torch.cuda.Stream() for _ in qs]
+    for _ in range(5):
+        for gr, st in zip(graphs, streams):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                gr.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(held, want):
+            assert torch.equal(a, b)

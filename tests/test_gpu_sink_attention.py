@@ -350,3 +350,56 @@ def test_scales_of_either_sign(fsi, dev, dtype, scale):
     q, k, v, dout = _inputs(1, 4, 2, 130, 130, 64, dtype, seed=12)
     got = _run(fsi, dev, q, k, v, dout, window=50, sinks=3, scale=scale)
     _check(got, *oracle.attention(q, k, v, dout, 50, 3, None, scale, *UNIT[dtype]))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_offsets_beyond_32_bits(fsi, dev, dtype):
+    """Rows 2^21 elements apart in one buffer of more than 2^31, and sequences 2^31 apart: as their copies."""
+    big = torch.zeros((1 << 31) + (1 << 23), dtype=dtype, device=dev)
+    far = big.as_strided((1, 2, 1024, 64), (0, 64, 1 << 21, 1))
+    seqs = big.as_strided((2, 2, 100, 64), (1 << 31, 64, 256, 1), 128)
+    g = torch.Generator().manual_seed(15)
+    for view in (far, seqs):
+        B, H, T, hd = view.shape
+        x = torch.randn(B, H, T, hd, generator=g).to(dtype).to(dev)
+        view.copy_(x)
+        q, _, _, dout = (t.to(dev) for t in _inputs(B, 4, H, T, T, hd, dtype, seed=T))
+        got, want = [], []
+        for kv, res in ((view, got), (x, want)):
+            leaves = [t.detach().requires_grad_() for t in (q, kv, kv)]
+            out = fsi.sink_window_attention(*leaves, window=70, sinks=3)
+            res += [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_two_backwards_at_once(fsi, dev, dtype):
+    """Calls on two streams at once, and graphs of them replayed on two, have workspaces of their own."""
+    sets = [[t.to(dev) for t in _inputs(1, 8, 2, 64, 2000, 64, dtype, seed=s)] for s in (1, 2)]
+
+    def step(q, k, v, dout):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = fsi.sink_window_attention(*leaves, window=1500, sinks=70)
+        return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+
+    want = [step(*s) for s in sets]
+    graphs, held = [], []
+    for s in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            held.append(step(*s))
+    streams = [torch.cuda.Stream() for _ in sets]
+    for i in range(6):
+        got = held
+        if i % 2:
+            got = [None, None]
+        for j, st in enumerate(streams):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                if i % 2:
+                    got[j] = step(*sets[j])
+                else:
+                    graphs[j].replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))

@@ -81,7 +81,8 @@ def test_sink_attention_errors(fsi):
                                None, 1.0, dtype, _ptr(4), 1, 1, 1, None, None, None, 0, None)
 
     def bwd(q=_ptr(1), Tq=3, Tk=5, hd=64, dtype=1, ws=None, nbytes=0, dk=_ptr(8)):
-        return L.fsi_sink_attn_bwd(q, 1, 1, 1, _ptr(2), 1, 1, 1, _ptr(3), 1, 1, 1, _ptr(4), 1, 1, 1, None, _ptr(5), 1, 1, 1,
+        return L.fsi_sink_attn_bwd(q, 1, 1, 1, _ptr(2), 1, 1, 1, _ptr(3), 1, 1, 1, _ptr(4), 1, 1, 1, None, _ptr(5),
+                                   1, 1, 1,
                                    _ptr(6), 1, 4, 2, Tq, Tk, hd, 2, 1, None, 1.0, dtype, _ptr(7), dk, _ptr(9), ws,
                                    nbytes, None)
 
@@ -122,6 +123,12 @@ def test_cache_constructor(fsi):
     with pytest.raises(ValueError, match="start positions"):
         c.load_dense(torch.zeros(1, 2, 1, 128).bfloat16(), torch.zeros(1, 2, 1, 128).bfloat16(),
                      start=torch.zeros(2, dtype=torch.int32))
+    for dt in (torch.float32, torch.bool):
+        with pytest.raises(TypeError, match="integers"):
+            c.load_dense(torch.zeros(1, 2, 1, 128).bfloat16(), torch.zeros(1, 2, 1, 128).bfloat16(),
+                         start=torch.zeros(1, dtype=dt))
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        c.to_dense(4)
     plain = make(kv_format=None)
     with pytest.raises(TypeError, match="kv_format"):
         plain.load_dense(torch.zeros(1, 2, 1, 128).bfloat16(), torch.zeros(1, 2, 1, 128).bfloat16(),
