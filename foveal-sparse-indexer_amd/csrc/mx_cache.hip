@@ -132,7 +132,9 @@ constexpr int MX_THREADS = 256;
 // A workgroup writes its share of one (page, head): a thread takes 8 dims of a token, a lane quad
 // a group.  K's codes go straight to memory (a token's row is contiguous); V's codes and both
 // scales are laid out in LDS, and leave as 16-byte pieces of a page that is written whole, as
-// single pairs and bytes otherwise.
+// single pairs and bytes otherwise.  Bound by bytes: 4 x 8192 tokens, 8 heads of 128, bf16 to 4 bits
+// (170 MB) take 31 - 35 us, 4.9 - 5.5 TB/s (with the read back 62 - 70; 364 with a wave per token and
+// single pairs for every page).
 template <typename T, int FMT, int HD>
 __global__ __launch_bounds__(MX_THREADS) void mx_write_kernel(MxParams P) {
   constexpr int BITS = MxFmt<FMT>::BITS, W2 = 2 * BITS / 8, NG = HD / MX_GROUP, TPT = HD / 8;
@@ -207,7 +209,8 @@ __global__ __launch_bounds__(MX_THREADS) void mx_write_kernel(MxParams P) {
 }
 
 // One page of a head back to rows: V's block through LDS, 8 dims of a token a thread.  0 where
-// the page is not there.
+// the page is not there.  The same 170 MB back take 26 - 27 us, 6.3 - 6.5 TB/s (the pages still lie
+// in the cache after the write).
 template <typename T, int FMT, int HD>
 __global__ __launch_bounds__(MX_THREADS) void mx_read_kernel(MxParams P) {
   constexpr int BITS = MxFmt<FMT>::BITS, W2 = 2 * BITS / 8, NG = HD / MX_GROUP, TPT = HD / 8;

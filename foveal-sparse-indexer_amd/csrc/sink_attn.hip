@@ -458,11 +458,13 @@ SkSinkSplit sk_split(int64_t Tq, int64_t Tk, int64_t window, int64_t sinks) {
 }
 
 // Whether `cols` columns of `heads` (sequence, head) pairs go to SPLIT workgroups: where workgroups
-// of 64 are fewer than the chip's CUs.
+// of 64 are fewer than the chip's CUs.  fp32, 3 sequences of 333, 6 / 3 heads of 64, with gradients:
+// 261 us in workgroups of 64, 159 split (of which the kernels 17 + 26 + 31, the rest is the host).
 bool sk_split_waves(int64_t cols, int64_t heads) { return (cols + SK_T - 1) / SK_T * heads < 256; }
 
 // Parts that the keys of `blocks` workgroups are cut into: as many as two workgroups a CU hold, each
-// of 4 key tiles at least.
+// of 4 key tiles at least.  32 / 8 heads, 1 query over 8192 keys, forward us in one part / cut: bf16
+// 199 / 39, fp32 410 / 68.
 constexpr int64_t SK_SLOTS = 512;
 int sk_key_splits(const SkParams& P, int64_t blocks, int64_t columns) {
   const int64_t span = std::min<int64_t>(P.Tk, static_cast<int64_t>(P.window) + columns);
@@ -481,7 +483,8 @@ size_t sk_part_bytes(const SkParams& P, int splits) {
                     : 0;
 }
 // Parts that the query heads of a KV head are cut into for dK and dV: while the key tiles leave CUs
-// without a workgroup.  unit: keys of a workgroup.
+// without a workgroup.  unit: keys of a workgroup.  8 heads on one KV head, 2048 tokens, window 1024,
+// bf16, forward and gradients: 508 us in one part, 174 cut.
 int sk_head_splits(const SkParams& P, const SkSinkSplit& S, int64_t unit, int64_t slots) {
   const int64_t far = S.parts ? (P.sinks + unit - 1) / unit * S.parts : 0;
   const int64_t blocks = ((P.Tk + unit - 1) / unit + far) * P.Hkv * P.B;

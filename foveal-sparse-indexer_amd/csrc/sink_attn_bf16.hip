@@ -63,6 +63,10 @@ __device__ __forceinline__ SbKeys sb_keys(const SkParams& P, int len, int a, int
 // The running maximum moves only when a score exceeds it by more than 2^8: P then stays below
 // 2^8, most tiles need one compare instead of the row maxima, and the accumulators are rescaled
 // rarely.
+// Bound: the matrix pipe, 0.72 of a large library product's rate; a tile's softmax stands beside
+// the other wave's products only.  16384 tokens, window 4096, 32 / 8 heads of 128 (963 GFLOP): 947 - 968
+// us, 995 - 1017 TFLOP/s.  Slower: 32 keys of a tile at a time 1045, the next tile's scores before
+// this one's softmax (spills) 7000, every K fragment read first 985.
 // ---------------------------------------------------------------------------
 constexpr int SB_THREADS = 256;
 constexpr int SB_WAVES = SB_THREADS / 64;
@@ -241,7 +245,8 @@ __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_fwd_kernel(SkPar
 
 // ---------------------------------------------------------------------------
 // dQ, and D for the key kernel.  A workgroup of 4 waves is HPW query heads of one KV head at
-// 64 * 2 / HPW queries; a wave is one head's 32 queries over 32 keys at a time.
+// 64 * 2 / HPW queries; a wave is one head's 32 queries over 32 keys at a time.  2 x 4096 tokens, window
+// 1024, 32 / 8 heads of 128: 200 us for 6 hd flops a pair (900 TFLOP/s); dS in two terms 235.
 // ---------------------------------------------------------------------------
 template <int HD, int HPW, bool FINE>
 __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_dq_kernel(SkParams P) {
@@ -383,7 +388,8 @@ __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_dq_kernel(SkPara
 
 // ---------------------------------------------------------------------------
 // dK and dV of 64 keys: wave (query half, key half) owns 32 keys and, of every query tile, 32
-// queries; the two query halves' sums meet in LDS at the end.
+// queries; the two query halves' sums meet in LDS at the end.  The same case: 278 us for 8 hd
+// flops a pair (870 TFLOP/s); dS in two terms 367 at best, the registers then hold no more.
 // The first S.tiles * S.parts workgroups of a KV head are the split sink tiles' (SkSinkSplit).
 // ---------------------------------------------------------------------------
 template <int HD, bool FINE>
