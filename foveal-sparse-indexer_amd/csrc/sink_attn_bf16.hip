@@ -63,15 +63,53 @@ __device__ __forceinline__ SbKeys sb_keys(const SkParams& P, int len, int a, int
 // The running maximum moves only when a score exceeds it by more than 2^8: P then stays below
 // 2^8, most tiles need one compare instead of the row maxima, and the accumulators are rescaled
 // rarely.
-// Bound: the matrix pipe, 0.72 of a large library product's rate; a tile's softmax stands beside
-// the other wave's products only.  16384 tokens, window 4096, 32 / 8 heads of 128 (963 GFLOP): 947 - 968
-// us, 995 - 1017 TFLOP/s.  Slower: 32 keys of a tile at a time 1045, the next tile's scores before
+// Bound: issue of the matrix pipe (0.48 busy) and the vector units (0.4), whose phases of a tile
+// overlap with the other wave's only.  16384 tokens, window 4096, 32 / 8 heads of 128 (963 GFLOP): 902
+// - 952 us card by card, 1010 - 1067 TFLOP/s; 2 x 4096, window 1024, with lse and remainder 167 - 179.
+// One test of both query tiles' maxima and the copies' offsets in registers: 943 -> 902, 178 -> 167.
+// Slower: 32 keys of a tile at a time 1045, the next tile's scores before
 // this one's softmax (spills) 7000, every K fragment read first 985.
 // ---------------------------------------------------------------------------
 constexpr int SB_THREADS = 256;
 constexpr int SB_WAVES = SB_THREADS / 64;
 // Workgroups a CU that a kernel's registers and LDS are kept to: head_dim 256 takes all of one.
 constexpr int sb_blocks(int hd) { return hd > 128 ? 1 : 2; }
+
+// sab_dma's copy of rows [r0, r0 + 64) by the workgroup, with what it needs of a thread kept in
+// registers: lo, the thread's byte offset from a row of its group of ROWS rows, and the wave's share of
+// the tile.  Bases are scalars of their own per group (opaque, or the compiler chains 64-bit vector
+// additions from one to the next).
+template <int HD>
+struct SbLoad {
+  static constexpr int PC = HD / 8, ROWS = SB_THREADS / PC, N = SK_T / ROWS;
+  int row, piece, wave;
+  __device__ __forceinline__ SbLoad() {
+    row = static_cast<int>(threadIdx.x) / PC;
+    piece = 16 * ((static_cast<int>(threadIdx.x) % PC) ^ sab_swz<HD>(row));
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  }
+  __device__ __forceinline__ void operator()(const bf16_t* base, int64_t rs, int r0, int T, char* tile) const {
+    const uint32_t rsb = static_cast<uint32_t>(rs) * 2u;
+    const char* rb = reinterpret_cast<const char*>(base + static_cast<int64_t>(r0) * rs);
+    char* dst = tile + wave * 1024;
+    if (r0 + SK_T <= T) {
+      const uint32_t lo = static_cast<uint32_t>(row) * rsb + static_cast<uint32_t>(piece);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const char* p = rb + static_cast<uint64_t>(j * ROWS) * rsb;
+        asm volatile("" : "+s"(p));
+        __builtin_amdgcn_global_load_lds((ab_glb_t*)(p + lo), (ab_lds_t*)(dst + j * SB_THREADS * 16), 16, 0, 0);
+      }
+    } else {
+      const int last = T - 1 - r0;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const uint32_t lo = static_cast<uint32_t>(min(j * ROWS + row, last)) * rsb + static_cast<uint32_t>(piece);
+        __builtin_amdgcn_global_load_lds((ab_glb_t*)(rb + lo), (ab_lds_t*)(dst + j * SB_THREADS * 16), 16, 0, 0);
+      }
+    }
+  }
+};
 
 template <int HD, int HPW, bool LSE>
 __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_fwd_kernel(SkParams P) {
@@ -92,11 +130,12 @@ __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_fwd_kernel(SkPar
   const bf16_t* v = static_cast<const bf16_t*>(P.v) + b * P.vs_b + g * P.vs_h;
   const SkTiles tiles = sk_key_tiles(P, off + i0, min(off + min(i0 + QW, P.Tq), len) - 1);
   const SkRange range = sk_key_part(P, tiles.count(), blockIdx.z);
+  const SbLoad<HD> copy;
   auto load = [&](int c) {
     if (c >= range.hi) return;
     char* dst = smem + (c & 1) * (2 * TB);
-    sab_dma<HD, SB_THREADS>(k, P.ks_t, tiles.tile(c) * SK_T, len, dst);
-    sab_dma<HD, SB_THREADS>(v, P.vs_t, tiles.tile(c) * SK_T, len, dst + TB);
+    copy(k, P.ks_t, tiles.tile(c) * SK_T, len, dst);
+    copy(v, P.vs_t, tiles.tile(c) * SK_T, len, dst + TB);
   };
   load(range.lo);
   u32x4_t q[2][KS];
@@ -139,11 +178,9 @@ __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_fwd_kernel(SkPar
         st[1][t] = mfma16x16x32(a, q[1][ks], st[1][t]);
       }
     }
-    u32x4_t pb[2][2];
-    float alpha[2];
+    if (all != SB_ALL) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (all != SB_ALL) {
+      for (int i = 0; i < 2; ++i) {
         const int lo = hi[i] - P.window;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
@@ -153,23 +190,35 @@ __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_fwd_kernel(SkPar
             st[i][t][j] = s <= hi[i] && (s > lo || s < P.sinks) ? st[i][t][j] : -INFINITY;
           }
       }
-      float mx = max3_raw(st[i][0][0], st[i][0][1], st[i][0][2]);
-      mx = max3_raw(mx, st[i][0][3], st[i][1][0]);
-      mx = max3_raw(mx, st[i][1][1], st[i][1][2]);
-      mx = max3_raw(mx, st[i][1][3], st[i][2][0]);
-      mx = max3_raw(mx, st[i][2][1], st[i][2][2]);
-      mx = max3_raw(mx, st[i][2][3], st[i][3][0]);
-      mx = max3_raw(mx, st[i][3][1], st[i][3][2]);
-      mx = max3_raw(mx, st[i][3][3], st[i][3][3]);
-      alpha[i] = 1.f;
-      if (__ballot(mx > thr[i]) != 0) {
-        const float cand = max_rows4(mx) * sl2;
+    }
+    float mx[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float a = max3_raw(st[i][0][0], st[i][0][1], st[i][0][2]), c2 = max3_raw(st[i][2][0], st[i][2][1], st[i][2][2]);
+      a = max3_raw(a, st[i][0][3], st[i][1][0]);
+      c2 = max3_raw(c2, st[i][2][3], st[i][3][0]);
+      a = max3_raw(a, st[i][1][1], st[i][1][2]);
+      c2 = max3_raw(c2, st[i][3][1], st[i][3][2]);
+      mx[i] = max3_raw(max3_raw(a, st[i][1][3], c2), st[i][3][3], st[i][3][3]);
+    }
+    if (__ballot(mx[0] > thr[0] || mx[1] > thr[1]) != 0) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float cand = max_rows4(mx[i]) * sl2;
         const bool bump = cand > m[i] + 8.f;
         const float m_new = bump ? cand : m[i];
-        alpha[i] = bump ? __builtin_amdgcn_exp2f(m[i] - m_new) : 1.f;
+        const float alpha = bump ? __builtin_amdgcn_exp2f(m[i] - m_new) : 1.f;
         m[i] = m_new;
         thr[i] = (m_new + 8.f) * inv_sl2;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[i][dt] *= alpha;
+        lsum[i] *= alpha;
+        l_full[i] *= alpha;
       }
+    }
+    u32x4_t pb[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
       float add[2] = {0.f, 0.f};
 #pragma unroll
       for (int hc = 0; hc < 2; ++hc)
@@ -181,15 +230,8 @@ __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_fwd_kernel(SkPar
           pb[i][hc][w] = bf_cvt2(pa, pc);
           if (LSE) add[w & 1] += pa + pc;
         }
-      if (LSE) l_full[i] = fmaf(l_full[i], alpha[i], add[0] + add[1]);
+      if (LSE) l_full[i] += add[0] + add[1];
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (__ballot(alpha[i] != 1.f) != 0) {
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) acc[i][dt] *= alpha[i];
-        lsum[i] *= alpha[i];
-      }
 #pragma unroll
     for (int hc = 0; hc < 2; ++hc) {
 #pragma unroll
@@ -246,7 +288,8 @@ __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_fwd_kernel(SkPar
 // ---------------------------------------------------------------------------
 // dQ, and D for the key kernel.  A workgroup of 4 waves is HPW query heads of one KV head at
 // 64 * 2 / HPW queries; a wave is one head's 32 queries over 32 keys at a time.  2 x 4096 tokens, window
-// 1024, 32 / 8 heads of 128: 200 us for 6 hd flops a pair (900 TFLOP/s); dS in two terms 235.
+// 1024, 32 / 8 heads of 128: 201 us for 6 hd flops a pair (900 TFLOP/s); dS in two terms 235.  The
+// next 32 keys' scores beside this half's exponents (whole tiles, in one block): 219 - 231 us.
 // ---------------------------------------------------------------------------
 template <int HD, int HPW, bool FINE>
 __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_dq_kernel(SkParams P) {
@@ -265,11 +308,12 @@ __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_dq_kernel(SkPara
   const bf16_t* v = static_cast<const bf16_t*>(P.v) + b * P.vs_b + g * P.vs_h;
   const SkTiles tiles = sk_key_tiles(P, off + i0, min(off + min(i0 + QW, P.Tq), len) - 1);
   const SkRange range = sk_key_part(P, tiles.count(), blockIdx.z);
+  const SbLoad<HD> copy;
   auto load = [&](int c) {
     if (c >= range.hi) return;
     char* dst = smem + (c & 1) * (2 * TB);
-    sab_dma<HD, SB_THREADS>(k, P.ks_t, tiles.tile(c) * SK_T, len, dst);
-    sab_dma<HD, SB_THREADS>(v, P.vs_t, tiles.tile(c) * SK_T, len, dst + TB);
+    copy(k, P.ks_t, tiles.tile(c) * SK_T, len, dst);
+    copy(v, P.vs_t, tiles.tile(c) * SK_T, len, dst + TB);
   };
   load(range.lo);
   u32x4_t q[2][KS], gr[2][KS];
@@ -352,6 +396,7 @@ __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_dq_kernel(SkPara
 #pragma unroll
           for (int j = 0; j < 4; ++j)  // dS^T
             dp[i][t][j] = __builtin_amdgcn_exp2f(fmaf(st[i][t][j], sl2, -lse[i])) * (dp[i][t][j] - dd[i]);
+      __builtin_amdgcn_iglp_opt(0);  // LDS reads spread between the products: 207 -> 201 us (the case above)
       u32x4_t ds[2], dl[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) sb_round<FINE>(dp[i][0], dp[i][1], ds[i], dl[i]);
@@ -388,8 +433,8 @@ __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_dq_kernel(SkPara
 
 // ---------------------------------------------------------------------------
 // dK and dV of 64 keys: wave (query half, key half) owns 32 keys and, of every query tile, 32
-// queries; the two query halves' sums meet in LDS at the end.  The same case: 278 us for 8 hd
-// flops a pair (870 TFLOP/s); dS in two terms 367 at best, the registers then hold no more.
+// queries; the two query halves' sums meet in LDS at the end.  The same case: 270 us for 8 hd
+// flops a pair (895 TFLOP/s); dS in two terms 367 at best, the registers then hold no more.
 // The first S.tiles * S.parts workgroups of a KV head are the split sink tiles' (SkSinkSplit).
 // ---------------------------------------------------------------------------
 template <int HD, bool FINE>
@@ -427,11 +472,12 @@ __global__ __launch_bounds__(SB_THREADS, sb_blocks(HD)) void sb_dkv_kernel(SkPar
   const uint32_t row_off = sab_row_off<HD>(r, kg) + 32 * wq * HD * 2;
   const uint32_t tr_off = sab_tr_off<HD>(r, kg) + 32 * wq * HD * 2;
   const float sl2 = P.scale * SB_LOG2E;
+  const SbLoad<HD> copy;
   auto load = [&](int i, int hh, int stage) {
     char* dst = smem + stage * STAGE;
     const int h = g * G + hh;
-    sab_dma<HD, SB_THREADS>(static_cast<const bf16_t*>(P.q) + b * P.qs_b + h * P.qs_h, P.qs_t, i, q_end, dst);
-    sab_dma<HD, SB_THREADS>(static_cast<const bf16_t*>(P.dout) + b * P.ds_b + h * P.ds_h, P.ds_t, i, q_end, dst + TB);
+    copy(static_cast<const bf16_t*>(P.q) + b * P.qs_b + h * P.qs_h, P.qs_t, i, q_end, dst);
+    copy(static_cast<const bf16_t*>(P.dout) + b * P.ds_b + h * P.ds_h, P.ds_t, i, q_end, dst + TB);
     if (wave < 2) {
       const float* st = (wave ? P.dd : P.lse) + (static_cast<int64_t>(b) * P.Hq + h) * P.Tq + min(i + lane, q_end - 1);
       __builtin_amdgcn_global_load_lds((ab_glb_t*)st, (ab_lds_t*)(dst + 2 * TB + wave * AB_T * 4), 4, 0, 0);
