@@ -655,8 +655,13 @@ void sb_forward(const SkParams& P, hipStream_t st) {
 // heads of 512 tokens (64 tiles) 27.8 / 29.8; heads of 128, (4, 4 heads, 27) 13.6 / 14.6, 8 heads of 512
 // 39.7 / 46.7.  Beyond, the product would be paid for in full: (1, 16 / 4 heads, 2048, 128) 151 / 190.
 constexpr int SB_FINE_TILES = 64;
+// Queries of up to SB_FINE_KEYS keys are too: the roundings of few terms do not average out (1 + 4 keys,
+// 21 heads of 3160: 2.5e-3 against 1.8e-3), for a third more time (2 x 4096, 32 / 8 heads of 128, window
+// 32: 179 / 247 us).
+constexpr int SB_FINE_KEYS = 16;
 static bool sb_fine(const SkParams& P) {
-  return SB_FINE_TILES >= static_cast<int64_t>(P.B) * P.Hkv * ((P.Tk + SK_T - 1) / SK_T);
+  return SB_FINE_TILES >= static_cast<int64_t>(P.B) * P.Hkv * ((P.Tk + SK_T - 1) / SK_T) ||
+         SB_FINE_KEYS >= P.window + P.sinks;
 }
 
 void sb_backward(const SkParams& P, const SkSinkSplit& S, hipStream_t st) {
