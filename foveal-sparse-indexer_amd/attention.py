@@ -222,6 +222,8 @@ class FovealKVCache:
                 raise TypeError(f"{what}: per-sequence start positions need a cache with a kv_format")
             if start.is_floating_point() or start.dtype == torch.bool:
                 raise TypeError(f"{what}: start positions must be integers, got {start.dtype}")
+            if start.dtype == torch.int64:  # beyond int32 is outside the cache, whatever its low bits are
+                start = start.clamp(-(1 << 31), (1 << 31) - 1)
             rows = start.to(device=self.k_cache.device, dtype=torch.int32).reshape(-1).contiguous()
             if rows.numel() != B:
                 raise ValueError(f"{what}: {rows.numel()} start positions for {B} sequences")
@@ -273,7 +275,7 @@ class FovealKVCache:
         """Write (B, Hkv, n, hd) K/V at positions start .. start + n - 1 (the
         reference layout) without touching the 16-D page state.  With a kv_format,
         start may be a (B,) integer tensor, one position per sequence; tokens outside the
-        cache are then skipped and reported as the other device-side index errors are."""
+        cache's pages are then skipped and reported as the other device-side index errors are."""
         self._write(k, v, start)
 
     def to_dense(self, n_tok: Optional[int] = None, batch: Optional[slice] = None):

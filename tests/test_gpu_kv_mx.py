@@ -404,3 +404,18 @@ def test_two_graphs_replayed_side_by_side(fsi, dev):
         torch.cuda.synchronize()
         for a, b in zip(held, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("start", [(1 << 32) + 3, -(1 << 32) + 3, (1 << 31) - 1, -(1 << 31)])
+def test_start_positions_beyond_32_bits(fsi, dev, fmt, start):
+    """Outside the cache, not wrapped into it."""
+    from foveal_sparse_indexer_amd import _lib
+
+    c = _cache(fsi, dev, 2, 64, 1, 64, F32, fmt)
+    x = torch.ones(2, 1, 2, 64, device=dev)
+    c.load_dense(x, x, start=torch.tensor([start, 5], device=dev))
+    ko, vo = c.to_dense(64)
+    assert (ko[0] == 0).all() and (vo[0] == 0).all() and (ko[1, :, 5:7] == 1).all() and int((ko[1] != 0).sum()) == 128
+    with pytest.raises(IndexError):
+        _lib.raise_device_errors(dev, "write")
